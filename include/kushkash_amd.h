@@ -196,7 +196,7 @@ int kush_combine_ex(int head_dim, int group, int dtype, void* out, const float* 
  * reference raises the driver's error string directly (_cuda.py:39-43). */
 const char* kush_last_error(void);
 
-/* ABI revision of this header (9) and of kushkash_amd_attend.h. No reference counterpart. */
+/* ABI revision of this header (10) and of kushkash_amd_attend.h, kushkash_amd_window.h and kushkash_amd_step.h. No reference counterpart. */
 int kush_abi_version(void);
 
 #ifdef __cplusplus

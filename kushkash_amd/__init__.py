@@ -5,9 +5,12 @@ Drop-in for the reference's kushkash.KushCache / kushkash._ops.Ops on one GPU, f
 entry points (KushHFCache, enable, generate; transformers is imported on first use) and for its
 SGLang plugin (kushkash_amd.sglang; SGLang is imported when the plugin registers)."""
 from ._ops import PAGE, Ops, record_bytes
+from ._step import MapSizes, StepMaps, block_table, map_sizes, sample, step_maps
+from ._window import window_attention
 from .cache import KushCache, MemoryStats
 
-__all__ = ["KushCache", "MemoryStats", "PAGE", "Ops", "record_bytes", "KushHFCache", "enable", "generate", "build"]
+__all__ = ["KushCache", "MemoryStats", "PAGE", "Ops", "record_bytes", "KushHFCache", "enable", "generate", "build",
+           "window_attention", "block_table", "step_maps", "map_sizes", "StepMaps", "MapSizes", "sample"]
 __version__ = "0.1.0"
 
 

@@ -64,8 +64,19 @@ def takes(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> bo
     return True
 
 
+def takes_out(out: torch.Tensor) -> bool:
+    """Whether the kernel can write this output in place: 16-byte aligned rows, dims adjacent."""
+    return (_plain(out) and out.stride(-1) == 1 and out.data_ptr() % 16 == 0
+            and not any(s % 8 or s < 0 for s in _row_strides(out, out.shape[-1])))
+
+
+def window_tiles(window: int, sinks: int, rows: int, group: int) -> int:
+    """The most key tiles that a row tile of `rows` rows sees under a window (csrc/kush_attend.hip)."""
+    return -(-sinks // KEYS) + (window + (rows - 1) // group) // KEYS + 2
+
+
 def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
-         scratch: int = PARTIAL_BYTES) -> tuple[int, int]:
+         scratch: int = PARTIAL_BYTES, window: int = 0, sinks: int = 0) -> tuple[int, int]:
     """(waves, chunk) of a call whose sequences have (T, N, count) query rows and keys. A row tile is 32 waves
     query rows (group heads of each token) of one kv head; 4 waves fill half a CU (a whole one at D 256, a
     quarter at D 64), 8 a whole one.
@@ -83,8 +94,11 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
                2-32 % slower than whole (3,072 tokens over themselves: 101 -> 129 us, 2,048 at D 64: 43 -> 52), with
                it 7 (up to 13 %), and 9 of the splits that it leaves out would have gained 2-13 %.
                Not below 24 tiles (1,000 tokens over themselves: 31 us whole, 31-34 split), and into no more parts
-               than min(scratch, PARTIAL_BYTES) holds the partials of."""
+               than min(scratch, PARTIAL_BYTES) holds the partials of.
+    With a window a row tile's keys are those that it sees, wherever they lie."""
     longest = max([n for _, n, _ in spans])
+    if window:
+        longest = min(longest, window_tiles(window, sinks, 128, group) * KEYS)
     nt = -(-longest // KEYS)
     if nt < 24:
         return 4, 0
@@ -96,7 +110,8 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
     for t, n, c in spans:
         tiles = -(-t * group // 128) * c
         tasks += tiles
-        units += tiles * -(-(n - t // 2 if causal else n) // KEYS)       # (causal: the mean over the rows, N >= T)
+        keys = n - t // 2 if causal else n                                # (causal: the mean over the rows, N >= T)
+        units += tiles * -(-(min(keys, longest) if window else keys) // KEYS)
     tasks, units = tasks * hkv, units * hkv
     if not tasks:
         return 4, 0
@@ -117,35 +132,42 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float, lse: bool = False,
-           cu: tuple | None = None, spans=None, out: torch.Tensor | None = None, scratch: int = PARTIAL_BYTES):
+           cu: tuple | None = None, spans=None, out: torch.Tensor | None = None, scratch: int = PARTIAL_BYTES,
+           window: int = 0, sinks: int = 0):
     """Attention of inputs that takes() accepts: out in q's shape and type (the given one, its rows 16-byte
     aligned, or a new one), or with lse the pair (out fp32, lse fp32 [.., Hq]). cu = (cu_q, cu_k, max_q, max_k)
     and spans = [(T, N)] for packed rows: the offsets as int32 device tensors, the lengths on the host. scratch: the
-    bytes that partials of split keys may take."""
+    bytes that partials of split keys may take. window (causal calls): of the keys up to its own a query sees the last
+    `window` and the first `sinks` (0: all of them)."""
     D, Hq, Hk = q.shape[-1], q.shape[-2], k.shape[-2]
     group = Hq // Hk
     if cu is None:
         seqs, n_q, n_k, total = q.shape[0], q.shape[1], k.shape[1], q.shape[0] * q.shape[1]
         cq = ck = None
-        waves, chunk = plan(((n_q, n_k, seqs),), group, Hk, D, total, causal, scratch)
+        window = 0 if window >= n_k else window
+        waves, chunk = plan(((n_q, n_k, seqs),), group, Hk, D, total, causal, scratch, window, sinks)
     else:
         cq, ck, n_q, n_k = cu[0].data_ptr(), cu[1].data_ptr(), cu[2], cu[3]
         seqs, total = len(spans), q.shape[0]
-        waves, chunk = plan([(t, n, 1) for t, n in spans], group, Hk, D, total, causal, scratch)
+        window = 0 if window >= n_k else window
+        waves, chunk = plan([(t, n, 1) for t, n in spans], group, Hk, D, total, causal, scratch, window, sinks)
     dev = q.device
     if out is None:
         out = torch.empty(q.shape, dtype=torch.float32 if lse else q.dtype, device=dev)
     logs = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if lse else None
     ls = _row_strides(logs.unsqueeze(-1), 1) if lse else (0, 0, 0)
     strides = _Strides(*_row_strides(q, D), *_row_strides(k, D), *_row_strides(v, D), *_row_strides(out, D), *ls)
-    rows = -(-(-(-n_k // KEYS)) // chunk) * total * Hq if chunk else 0          # partial rows: every split's
+    tiles = -(-n_k // KEYS) if not window else min(-(-n_k // KEYS), window_tiles(window, sinks, 32 * waves, group))
+    rows = -(-tiles // chunk) * total * Hq if chunk else 0                     # partial rows: every split's
     part = torch.empty(rows * (D + 2), dtype=torch.float32, device=dev) if chunk else None
+    name = "kush_window_attend" if window else "kush_attend"
+    limit = (window, sinks) if window else ()
     with torch.cuda.device(dev):
-        rc = _lib.lib().kush_attend(
+        rc = getattr(_lib.lib(), name)(
             D, 1 if q.dtype == torch.float16 else 2, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             logs.data_ptr() if lse else None, ctypes.addressof(strides), cq, ck, n_q, n_k, total, seqs, Hk, group, scale,
-            int(causal), int(lse), waves, chunk, part.data_ptr() if chunk else None,
-            part.data_ptr() + rows * D * 4 if chunk else None, torch.cuda.current_stream(dev).cuda_stream)
+            *(() if window else (int(causal),)), int(lse), waves, chunk, part.data_ptr() if chunk else None,
+            part.data_ptr() + rows * D * 4 if chunk else None, torch.cuda.current_stream(dev).cuda_stream, *limit)
     if rc:
-        raise RuntimeError(f"kush_attend failed ({rc}): {(_lib.lib().kush_last_error() or b'').decode(errors='replace')}")
+        raise RuntimeError(f"{name} failed ({rc}): {(_lib.lib().kush_last_error() or b'').decode(errors='replace')}")
     return (out, logs) if lse else out

@@ -14,9 +14,10 @@ from pathlib import Path
 import torch   # noqa: F401  -- loads torch's HIP runtime first; the library binds to it (same soname)
 
 LIB = Path(__file__).resolve().parent / "libkushhip.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_F64 = ctypes.c_double
 
 # head_dim, bits, dtype, k, v, k_row_stride, v_row_stride, seq_lens, pos_offset, advance, tail_idx, cache,
 # block_stride, head_stride, tail_k, block_table, bt_row_stride, hkv, n_seqs, stream
@@ -63,6 +64,25 @@ ATTEND_SIGNATURES = {
     "kush_attend": [_I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F, _I32, _I32, _I32,
                     _I32, _P, _P, _P],
 }
+# include/kushkash_amd_window.h
+WINDOW_SIGNATURES = {
+    # the decode list, then k, v, k_row_stride, v_row_stride, split_sync, waves, seq_order, rot, window, sinks
+    "kush_window_decode": _DECODE + [_P, _P, _I64, _I64, _P, _I32, _P, _I32, _I32, _I32],
+    # kush_attend's list without causal, then window, sinks
+    "kush_window_attend": [_I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F, _I32, _I32,
+                           _I32, _P, _P, _P, _I32, _I32],
+}
+# include/kushkash_amd_step.h
+STEP_SIGNATURES = {
+    # req_to_token, map_row_stride, map_rows, map_cols, req, wide_req, seq_lens, wide_lens, n_reqs, pages, table,
+    # table_row_stride, lens_out, slots_out, stream
+    "kush_block_table": [_P, _I64, _I64, _I64, _P, _I32, _P, _I32, _I64, _I64, _P, _I64, _P, _P, _P],
+    # new_tokens, history, slots, block_table, bt_row_stride, bt_cols, n_reqs, window, sinks, jobs, pages, tails, tokens,
+    # the eleven outputs, stream
+    "kush_step_maps": [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I64, _I64, _I64, _I64] + [_P] * 12,
+    # dtype, logits, row_stride, rows, vocab, uniforms, then (value, per row) of temperature, top_k, top_p, min_p; out, stream
+    "kush_sample": [_I32, _P, _I64, _I64, _I64, _P, _F64, _P, _I32, _P, _F64, _P, _F64, _P, _P, _P],
+}
 
 
 @lru_cache(None)
@@ -74,7 +94,7 @@ def lib() -> ctypes.CDLL:
     if cdll.kush_abi_version() != ABI_VERSION:                  # before anything it may not export is looked up
         raise RuntimeError(f"kushkash_amd: {LIB.name} has ABI {cdll.kush_abi_version()}, expected {ABI_VERSION}; "
                            "rebuild it")
-    for name, args in (SIGNATURES | ATTEND_SIGNATURES).items():
+    for name, args in (SIGNATURES | ATTEND_SIGNATURES | WINDOW_SIGNATURES | STEP_SIGNATURES).items():
         fn = getattr(cdll, name)
         fn.argtypes = args
         fn.restype = ctypes.c_char_p if name == "kush_last_error" else ctypes.c_int32

@@ -28,7 +28,8 @@ from functools import lru_cache
 
 import torch
 
-PAGE = 32
+from ._window import PAGE, check_limit
+
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 DECODE_WAVES = 4                # default waves per decode workgroup (kush_decode: waves = 0)
 SYNC_SLOTS = 1 << 16            # split-K merge counters per Ops: (sequence, kv head, 16-head chunk) slots
@@ -241,10 +242,12 @@ class Ops:
         if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
             raise ValueError("block_table must be int32 [S, max_pages] with unit column stride")
 
-    def _check_values(self, cache, block_table, seq_lens, tail_idx, tail_k, rows: int, extra: int = 0) -> None:
+    def _check_values(self, cache, block_table, seq_lens, tail_idx, tail_k, rows: int, extra: int = 0, window: int = 0,
+                      sinks: int = 0) -> None:
         """Index ranges (one host sync; on when validate=True or KUSHKASH_AMD_VALIDATE=1): the kernels
         themselves do no bounds checks, as the reference's. extra: tokens added to seq_lens before the
-        pages are counted (append: pos_offset + 1; rows left at <= 0 tokens are padding)."""
+        pages are counted (append: pos_offset + 1; rows left at <= 0 tokens are padding). window, sinks: only the pages
+        that are seen need a valid block."""
         if rows == 0 or not self._validating():
             return
         lens = (seq_lens[:rows].long() + extra).clamp(min=0)
@@ -253,7 +256,10 @@ class Ops:
         if need > block_table.shape[1]:
             raise ValueError(f"block_table has {block_table.shape[1]} pages per sequence, {need} needed")
         if need:
-            used = torch.arange(need, device=block_table.device)[None, :] < pages[:, None]
+            page = torch.arange(need, device=block_table.device)[None, :]
+            used = page < pages[:, None]
+            if window:
+                used &= (page * PAGE < sinks) | (page >= ((lens - window).clamp(min=0) // PAGE)[:, None])
             ids = block_table[:rows, :need][used]
             if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= cache.shape[0]):
                 raise ValueError(f"block_table points outside the cache ({cache.shape[0]} blocks)")
@@ -423,10 +429,15 @@ class Ops:
                        new_dst.data_ptr(), n_new, kp.data_ptr(), vp.data_ptr(), int(bool(rot)), self._stream())
 
     # ---------------------------------------------------------------- decode
-    def splits(self, num_seqs: int, num_kv_heads: int, max_full_pages: int) -> int:
+    def splits(self, num_seqs: int, num_kv_heads: int, max_full_pages: int, *, window: int | None = None,
+               sinks: int = 0) -> int:
         """Split-K factor for MI355X, at most 256: 1 where the (sequence, kv head) pairs fill the CUs by themselves,
         else the count that _split_count estimates to be the fastest. The grid stays within two workgroups per
-        CU, as in the reference (_ops.py:182-189), so a work buffer of 2 CUs * G * (D + 2) floats always suffices."""
+        CU, as in the reference (_ops.py:182-189), so a work buffer of 2 CUs * G * (D + 2) floats always suffices.
+        window, sinks: of a decode that is limited so, whose pages are those it sees."""
+        window, sinks = check_limit(window, sinks)
+        if window:
+            max_full_pages = min(max_full_pages, -(-sinks // PAGE) + window // PAGE)
         if not self.gpu:                                         # the host decode takes no splits (1 on CPU)
             return 1
         return _split_count(self.sms, num_seqs * num_kv_heads * -(-self.G // 16), max_full_pages,
@@ -453,7 +464,8 @@ class Ops:
     def decode(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                seq_lens: torch.Tensor, tail_idx: torch.Tensor, tail_k: torch.Tensor,
                scale: float, n_splits: int = 1, work: torch.Tensor | None = None, *,
-               waves: int | None = None, order: torch.Tensor | None = None, rot: bool = False) -> None:
+               waves: int | None = None, order: torch.Tensor | None = None, rot: bool = False,
+               window: int | None = None, sinks: int = 0) -> None:
         """out[s] = attention of q[s] ([Hq, D]) over the seq_lens[s] cached tokens of sequence s.
         n_splits > 1 needs `work` (fp32, >= S*Hkv*n_splits*G*(D+2) elements) (_ops.py:191-213); the
         splits are merged inside the same launch (split-K counters of this Ops), or by a second
@@ -463,7 +475,15 @@ class Ops:
         lengths a serving engine's metadata builder holds); it does not change the results. Calls on
         one Ops must not run concurrently on different streams (they share the counters, as the
         reference's callers share `work`). rot: the cache was written with rot=True: q is rotated on
-        load and the output rotated back inside the kernels (no reference counterpart)."""
+        load and the output rotated back inside the kernels (no reference counterpart). window: q[s] sees the
+        last `window` of the tokens and the first `sinks` alone (on the GPU; no reference counterpart); the pages between
+        are not read and their block_table entries may be anything, and n_splits counts over the pages that are seen
+        (splits(window=, sinks=))."""
+        window, sinks = check_limit(window, sinks)
+        if window:
+            self._decode(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot,
+                         None, None, window, sinks)
+            return
         if self._native() and self._native_decode(None, None, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale,
                                                   n_splits, work, waves, order, rot):
             return
@@ -473,13 +493,16 @@ class Ops:
     def append_decode(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor, out: torch.Tensor,
                       cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, tail_idx: torch.Tensor,
                       tail_k: torch.Tensor, scale: float, n_splits: int = 1, work: torch.Tensor | None = None, *,
-                      waves: int | None = None, order: torch.Tensor | None = None, rot: bool = False) -> None:
+                      waves: int | None = None, order: torch.Tensor | None = None, rot: bool = False,
+                      window: int | None = None, sinks: int = 0) -> None:
         """append(k, v, ..., pos_offset=-1, advance=False) followed by decode(q, out, ...), in one launch
         when it applies (at most 16 q heads per kv head, 16-byte aligned k / v rows; otherwise the two
         calls): row s of k / v is the token at position seq_lens[s] - 1, which seq_lens already counts
-        (the serving engines' convention). The same bytes and outputs as the two calls. No reference
-        counterpart."""
-        if self._native() and self._native_decode(k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale,
+        (the serving engines' convention). The same bytes and outputs as the two calls. window, sinks: as in
+        decode. No reference counterpart."""
+        window, sinks = check_limit(window, sinks)
+        limit = {"window": window, "sinks": sinks} if window else {}
+        if not window and self._native() and self._native_decode(k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale,
                                                   n_splits, work, waves, order, rot):
             return
         S, H = q.shape[0], tail_k.shape[1]
@@ -492,14 +515,14 @@ class Ops:
         if self.G > 16 or not aligned or not self.gpu:
             self.append(k, v, seq_lens, tail_idx, cache, block_table, tail_k, -1, False, rot=rot)
             self.decode(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves=waves,
-                        order=order, rot=rot)
+                        order=order, rot=rot, **limit)
             return
         self._on_device(k=k, v=v)
         self._decode(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot,
-                     k, v)
+                     k, v, window, sinks)
 
     def _decode(self, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot,
-                app_k, app_v) -> None:
+                app_k, app_v, window: int = 0, sinks: int = 0) -> None:
         S, H = q.shape[0], tail_k.shape[1]
         G, D = self.G, self.D
         if q.shape != (S, H * G, D) or not q.is_contiguous() or q.dtype != self.dtype:
@@ -514,7 +537,8 @@ class Ops:
             raise ValueError("seq_lens, tail_idx and block_table need one entry per sequence")
         if n_splits < 1:
             raise ValueError("n_splits must be >= 1")
-        self._check_values(cache, block_table, seq_lens, tail_idx, tail_k, S)
+        self._check_values(cache, block_table, seq_lens, tail_idx, tail_k, S, window=window, sinks=sinks)
+        _require(self.gpu or not window, "a window is a GPU extension; the CPU path attends over every token")
         if not self.gpu:                # one pass per (sequence, kv head): splits, work, waves, order unused
             _require(not rot, "decode(rot=True) is a GPU extension; the CPU path takes a rotated q (fwht)")
             bs, hs = _byte_strides(cache)
@@ -547,7 +571,11 @@ class Ops:
                int(n_splits), part_ml, part_o, S, stream)
         ext = (min(block_table.shape[1], 1 << 30), sync, wv, order.data_ptr() if order is not None else None,
                int(bool(rot)))
-        if app_k is None:
+        if window:
+            rows = (None, None, 0, 0) if app_k is None else (app_k.data_ptr(), app_v.data_ptr(), app_k.stride(0),
+                                                             app_v.stride(0))
+            self._lib.call("kush_window_decode", *ref, *rows, *ext[1:], window, sinks)
+        elif app_k is None:
             self._lib.call("kush_decode_ex", *ref, *ext)
         else:
             self._lib.call("kush_append_decode", *ref, app_k.data_ptr(), app_v.data_ptr(), app_k.stride(0),

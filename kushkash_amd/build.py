@@ -38,8 +38,9 @@ FAST_LIB = PKG / "_fastcall.so"
 FAST_SOURCE = "kush_fastcall.cpp"
 FAST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 SOURCES = ("kush_capi.hip", "kush_write.hip", "kush_decode.hip", "kush_rotate.hip",
-           "kush_unpack.hip", "kush_attend.hip", "kush_decode_inst.hip")
-# the decode kernel instantiations: one object per (input dtype, rot)
+           "kush_unpack.hip", "kush_attend.hip", "kush_window_attend.hip", "kush_step.hip", "kush_decode_inst.hip",
+           "kush_window_inst.hip")
+# the decode kernel instantiations (without and with a window): one object per (input dtype, rot)
 DECODE_INST = [{"KUSH_INST_IN": t, "KUSH_INST_ROT": r} for t in ("float", "_Float16", "kush::bf16_t") for r in (0, 1)]
 
 
@@ -50,7 +51,7 @@ def units() -> list[tuple[str, dict]]:
     """(source, preprocessor defines) of every object of the library."""
     out = []
     for s in SOURCES:
-        out += [(s, d) for d in DECODE_INST] if s == "kush_decode_inst.hip" else [(s, {})]
+        out += [(s, d) for d in DECODE_INST] if s in ("kush_decode_inst.hip", "kush_window_inst.hip") else [(s, {})]
     return out
 ARCH = "gfx950"
 
@@ -121,7 +122,8 @@ def source_digest(unit: str | None = None) -> str:
     h = hashlib.sha256()
     if unit is None:
         files = sorted((PKG / "csrc").glob("*.h")) + sorted((PKG / "csrc").glob("*.hip"))
-        files += [ROOT / "include" / "kushkash_amd.h", ROOT / "include" / "kushkash_amd_attend.h"]
+        files += [ROOT / "include" / f for f in ("kushkash_amd.h", "kushkash_amd_attend.h",
+                                                "kushkash_amd_window.h", "kushkash_amd_step.h")]
     else:
         seen: set = set()
         _includes(PKG / "csrc" / unit, seen)

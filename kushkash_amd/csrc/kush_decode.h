@@ -1063,6 +1063,51 @@ __device__ void merge_splits(const float* __restrict__ part_ml, const float* __r
     __syncthreads();
 }
 
+// The pages that the query at position n - 1 sees, as a list: logical pages 0 .. first - 1 (the sinks'), then those
+// from first + gap on (the window's), so list index p stands for logical page p or p + gap. Tokens lo .. lo + count - 1 of
+// the list's tokens (32 p + t) are hidden: behind the sinks on their last page, before the window on its first.
+// Every page of the list holds a token that is seen. WN false: all pages, nothing hidden.
+template <bool WN>
+struct View {
+    static constexpr int gap = 0;
+    __device__ __forceinline__ View(int) {}
+    __device__ __forceinline__ int page(int p) const { return p; }
+    __device__ __forceinline__ bool hidden(int) const { return false; }
+};
+template <>
+struct View<true> {
+    int first, gap, lo;
+    uint32_t count;
+    __device__ __forceinline__ View(int n, int window, int sinks) {
+        const int begin = n > window ? n - window : 0;           // the window's first token
+        first = sinks / PAGE + (sinks % PAGE != 0);
+        gap = max(0, begin / PAGE - first);
+        lo = sinks;
+        count = (uint32_t)max(0, begin - gap * PAGE - sinks);
+    }
+    __device__ __forceinline__ int page(int p) const { return p < first ? p : p + gap; }
+    __device__ __forceinline__ bool hidden(int t) const { return (uint32_t)(t - lo) < count; }
+    // whether any of n tokens from t on are hidden
+    __device__ __forceinline__ bool hides(int t, int n) const { return count != 0 && lo < t + n && t < lo + (int)count; }
+    // scores of tokens t + tok(q, j), the hidden ones out of the softmax (whatever they are, NaN too)
+    __device__ __forceinline__ void mask(float (&sv)[8], int t, int q) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sv[j] = hidden(t + tok(q, j)) ? -__builtin_inff() : sv[j];
+    }
+    // V scale and bias of one token of a staged page zeroed: a hidden token's weight 0 must not meet an infinity or NaN
+    template <typename F>
+    __device__ __forceinline__ void clear_v(uint8_t* slot, int t) const {
+        *reinterpret_cast<uint16_t*>(slot + F::OFF_VS + 2 * t) = 0;
+        *reinterpret_cast<uint16_t*>(slot + F::OFF_VB + 2 * t) = 0;
+    }
+    // and of the hidden tokens of a staged pair (pages `step` bytes apart, tokens from t on), by the wave that staged it
+    template <typename F>
+    __device__ __forceinline__ void clear_v(uint8_t* s0, int step, int t, int lane) const {
+        if (hidden(t + lane)) clear_v<F>(s0 + (lane / PAGE) * step, lane % PAGE);
+        asm volatile("" ::: "memory");
+    }
+};
+
 // grid (S, Hkv, n_splits * ceil(G / 16)), block NW * 64. Registers are budgeted for two waves per SIMD
 // (amdgpu_waves_per_eu(2); naming a maximum too changes no instruction; the library is built with MFMA accumulators in VGPRs): with a 512-register
 // budget the 4-wave variant used 236 VGPRs + 76 AGPRs and spent 46 v_accvgpr moves per page in its
@@ -1071,15 +1116,20 @@ __device__ void merge_splits(const float* __restrict__ part_ml, const float* __r
 // NS > 1: each workgroup writes its split's partials; with `sync` (one zeroed int32 per
 // (sequence, kv head, head chunk)), the last workgroup of a (sequence, kv head, head chunk) to
 // finish merges all splits into `out` and resets its counter, so no second launch is needed.
-template <int D, int BITS, typename IN, int NW, int ST, bool ROT, bool WS, int DEP>
+//
+// win = (window, sinks), or nothing: the query sees the last `window` tokens and the first `sinks` ones. The pages from
+// the sinks' last to the window's first are left out: the kernel runs over a list of the pages that are seen (View), and
+// what those two pages hold of hidden tokens is one run of the list's tokens, masked before the softmax.
+template <int D, int BITS, typename IN, int NW, int ST, bool ROT, bool WS, int DEP, typename... Win>
 __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D == 64 ? 4 : 2))) void decode_kernel(
     const IN* __restrict__ qg, IN* __restrict__ out, uint8_t* __restrict__ cache, int64_t bs, int64_t hs,
     IN* __restrict__ tail_k, const int32_t* __restrict__ tail_idx, const int32_t* __restrict__ block_table,
     const int32_t* __restrict__ seq_lens, int64_t bt_stride, int bt_cols, int H, int G, float p2, float rs, int NS,
     float* __restrict__ part_ml, float* __restrict__ part_o, int32_t* __restrict__ sync,
     const int32_t* __restrict__ seq_order, const IN* __restrict__ app_k, const IN* __restrict__ app_v, int64_t app_ks,
-    int64_t app_vs, int KW) {
-    constexpr bool ws = WS;
+    int64_t app_vs, int KW, Win... win) {
+    constexpr bool ws = WS, WN = sizeof...(Win) != 0;
+    static_assert(!WN || (!WS && DEP == 2), "a window runs with shared splits and two pairs per wave");
     using F = Fmt<D, BITS>;
     using R = Ring<D, BITS>;
     constexpr int KSTEPS = D / 32;
@@ -1179,7 +1229,7 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
     if (app_k != nullptr && zg == NSG - 1 && w == aw)
         token.load(app_k + (int64_t)s * app_ks + (int64_t)h * D, app_v + (int64_t)s * app_vs + (int64_t)h * D, lane);
     constexpr int PRE = WIN / (NW * WAVE);                               // prefetched ids per thread
-    const int npre = !ws && z == 0 ? min(WIN, bt_cols) : 0;
+    const int npre = !ws && !WN && z == 0 ? min(WIN, bt_cols) : 0;      // (WN: the pages depend on the length)
     int pre[PRE];
 #pragma unroll
     for (int k = 0; k < PRE; ++k) {
@@ -1189,7 +1239,8 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
 
     const int n = seq_lens[s];
     const int tix = tail_idx != nullptr ? tail_idx[s] : 0;              // the tail slot, with the length
-    const int full = n / PAGE, tail_n = n % PAGE;
+    const View<WN> view(n, win...);
+    const int full = n / PAGE - view.gap, tail_n = n % PAGE;            // full pages (of the list)
     const int pps = (full + NS - 1) / NS;
     const int p0 = min(full, z * pps), p1 = min(full, p0 + (ws ? KW : 1) * pps);
     const int wp1 = ws ? min(full, (zg + 1) * NW * KW * pps) : p1, wp0 = ws ? min(full, zg * NW * KW * pps) : p0;
@@ -1206,7 +1257,7 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
     if (app_k != nullptr && gc == 0 && n > 0) {
         const int pos = n - 1, slot = pos % PAGE, pg = pos / PAGE;
         if (slot == PAGE - 1) {
-            const int owner = pg / max(pps, 1);
+            const int owner = (pg - view.gap) / max(pps, 1);
             if (zg == (ws ? owner / (NW * KW) : owner)) {           // the whole workgroup
                 const IN* krow = app_k + (int64_t)s * app_ks + (int64_t)h * D;
                 IN* tail = tail_k + ((int64_t)tix * H + h) * PAGE * D;
@@ -1222,7 +1273,7 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
         }
     }
     const bool has_tail = tail_n > 0 && zg == NSG - 1;                 // the workgroup holds the last split
-    const int tail_blk = has_tail ? bt[full] : 0;                      // in before the page loop starts
+    const int tail_blk = has_tail ? bt[full + view.gap] : 0;           // in before the page loop starts
     const auto append_token = [&]() {
         if (appends && w == aw)
             token.template store<ROT>(tail_k + (((int64_t)tix * H + h) * PAGE + tail_n - 1) * D,
@@ -1313,7 +1364,7 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
 #pragma unroll
                 for (int k = 0; k < PRE; ++k) {
                     const int i = (int)threadIdx.x + k * NW * WAVE;
-                    ids[k] = i < wn ? bt[wb + i] : 0;
+                    ids[k] = i < wn ? bt[view.page(wb + i)] : 0;
                 }
 #pragma unroll
                 for (int k = 0; k < PRE; ++k) {
@@ -1403,12 +1454,16 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
         if ((P) >= pairs) break;                                                                   \
         KUSH_WAIT_VM((DEP - 1) * 2 * R::DMA);                                                      \
         if ((P) == 0) KUSH_MARK(2);                                                                \
+        if constexpr (WN) {                                                                        \
+            if (view.hides((wb + 2 * (P)) * PAGE, 2 * PAGE)) view.template clear_v<F>(SA, R::SLOT, (wb + 2 * (P)) * PAGE, lane); \
+        }                                                                                          \
         const int nx = (P) + DEP * PS;                   /* this wave's next pair in these slots */ \
         int2 id2;                                                                                  \
         if constexpr (ST == 2) {                                                                   \
             float sv[8], kx;                                                                       \
             pair_scores2<D, BITS, QLO>(SA, qa, qla, qh, ql, sv, kx, rs, lane);                     \
             if (2 * (P) + 1 >= wn && r16 >= 8) kx = -__builtin_inff();   /* page B masked */        \
+            if constexpr (WN) view.mask(sv, (wb + 2 * (P) + (r16 >> 3)) * PAGE, q);                \
             id2 = *reinterpret_cast<const int2*>(tb + min(2 * nx, TW - 2));                        \
             consume2<D, BITS, vpre<D, BITS, DEP, WS>()>(SA, R::SLOT, o, vacc, sv, sa, kx, m_run, l_run, vb_run, lane);       \
         } else {                                                                                   \
@@ -1421,6 +1476,10 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
             /* path)                                                                            */ \
             const float pbm = 2 * (P) + 1 >= wn ? -__builtin_inff() : 0.0f;                        \
             _Pragma("unroll") for (int jj = 0; jj < 8; ++jj) sv[1][jj] += pbm;                     \
+            if constexpr (WN) {                                                                    \
+                view.mask(sv[0], (wb + 2 * (P)) * PAGE, q);                                        \
+                view.mask(sv[1], (wb + 2 * (P) + 1) * PAGE, q);                                    \
+            }                                                                                      \
             id2 = *reinterpret_cast<const int2*>(tb + min(2 * nx, TW - 2));                        \
             consume_pages<D, BITS, 2, vpre<D, BITS, DEP, WS>()>(sp, o, vacc, sv, sa, kx, m_run, l_run, vb_run, lane);        \
         }                                                                                          \
@@ -1518,7 +1577,8 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
 #pragma unroll
         for (int e = 0; e < DS; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(qpk.get(e) * sm_log2, kpk.get(e), c, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[(kp * 16 + 4 * q + i) * PAGE + tt] = tt < tail_n ? c[i] : -__builtin_inff();
+        for (int i = 0; i < 4; ++i)
+            sc[(kp * 16 + 4 * q + i) * PAGE + tt] = tt < tail_n && !view.hidden(full * PAGE + tt) ? c[i] : -__builtin_inff();
         __syncthreads();
         if (w == tw) {
             float x[1][8];
@@ -1540,6 +1600,10 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
                     *reinterpret_cast<uint16_t*>(tslot + F::OFF_VS + 2 * (tail_n - 1)) = (uint16_t)sb;
                     *reinterpret_cast<uint16_t*>(tslot + F::OFF_VB + 2 * (tail_n - 1)) = (uint16_t)(sb >> 16);
                 }
+                asm volatile("" ::: "memory");
+            }
+            if constexpr (WN) {                                  // the hidden tokens' values, and what lies past the end
+                if (lane < PAGE && (lane >= tail_n || view.hidden(full * PAGE + lane))) view.template clear_v<F>(tslot, lane);
                 asm volatile("" ::: "memory");
             }
             if constexpr (ST == 2) {                             // stream 0 takes the page
@@ -1830,6 +1894,14 @@ int launch_decode(dim3 grid, hipStream_t stream, const void* q, void* out, const
                          const int32_t* seq_lens, int64_t bt_stride, int bt_cols, int hkv, int group, float p2, float rs,
                          int n_splits, float* part_ml, float* part_o, int32_t* sync, const int32_t* seq_order,
                          const void* app_k, const void* app_v, int64_t app_ks, int64_t app_vs, int ws);
+
+// The same with a window, instantiated in kush_window_inst.hip (2 and 4 waves)
+template <int D, int BITS, typename IN, int NW, bool ROT>
+int launch_window(dim3 grid, hipStream_t stream, const void* q, void* out, const void* cache, int64_t bs, int64_t hs,
+                  const void* tail_k, const int32_t* tail_idx, const int32_t* block_table, const int32_t* seq_lens,
+                  int64_t bt_stride, int bt_cols, int hkv, int group, float p2, float rs, int n_splits, float* part_ml,
+                  float* part_o, int32_t* sync, const int32_t* seq_order, const void* app_k, const void* app_v,
+                  int64_t app_ks, int64_t app_vs, int window, int sinks);
 
 #ifdef KUSH_DECODE_INSTANTIATE
 // Page pairs each wave holds in its ring where a third array fits (KUSHKASH_AMD_RING=2 | 3)

@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "kush_decode.h"
+#include "kushkash_amd_window.h"
 
 using namespace kush;
 
@@ -15,6 +16,11 @@ struct Append {
     const void* k = nullptr;
     const void* v = nullptr;
     int64_t k_stride = 0, v_stride = 0;
+};
+
+// What the query sees: all of its sequence (size 0), or its last `size` tokens and first `sinks` ones
+struct Window {
+    int32_t size = 0, sinks = 0;
 };
 
 // Wave splits (decode_kernel WS: every wave a whole split of its own, the workgroup's q and launch
@@ -49,7 +55,8 @@ int decode_impl(const char* what, int head_dim, int bits, int group, int dtype, 
                 const void* cache, int64_t block_stride, int64_t head_stride, const void* tail_k, const int32_t* tail_idx,
                 const int32_t* block_table, const int32_t* seq_lens, int64_t bt_stride, int32_t bt_cols, int32_t hkv,
                 float scale, int32_t n_splits, float* part_ml, float* part_o, int32_t* split_sync, int32_t waves,
-                const int32_t* seq_order, int32_t n_seqs, int32_t rot, const Append& app, void* stream) {
+                const int32_t* seq_order, int32_t n_seqs, int32_t rot, const Append& app, void* stream,
+                const Window& win = Window{}) {
     if (n_seqs < 0 || hkv <= 0 || group <= 0 || n_splits <= 0 || bt_cols < 0 || rot < 0 || rot > 1)
         return kush_fail(-2, "%s: bad n_seqs %d / hkv %d / group %d / n_splits %d / bt_cols %d / rot %d", what, n_seqs,
                          hkv, group, n_splits, bt_cols, rot);
@@ -86,12 +93,19 @@ int decode_impl(const char* what, int head_dim, int bits, int group, int dtype, 
         // the largest of the requested, 4 and 2 waves whose rings fit in LDS
         const auto launch = [&](auto nw) -> int {
             constexpr int NW = decltype(nw)::value;
+            if (win.size > 0) {
+                if constexpr (NW <= 4) {
+                    const dim3 g(n_seqs, hkv, n_splits * n_gc);
+                    return rot ? launch_window<D, BITS, IN, NW, true>(g, KUSH_DECODE_ARGS, win.size, win.sinks)
+                               : launch_window<D, BITS, IN, NW, false>(g, KUSH_DECODE_ARGS, win.size, win.sinks);
+                }
+            }
             const int ws = wave_splits(n_splits, NW, (int64_t)n_seqs * hkv * n_gc, split_sync != nullptr);
             const dim3 g(n_seqs, hkv, (ws ? n_splits / (NW * ws) : n_splits) * n_gc);
             return rot ? launch_decode<D, BITS, IN, NW, true>(g, KUSH_DECODE_ARGS, ws)
                        : launch_decode<D, BITS, IN, NW, false>(g, KUSH_DECODE_ARGS, ws);
         };
-        if (waves >= 8) {
+        if (waves >= 8 && win.size == 0) {
             if constexpr (decode_fits<D, BITS, 8>()) return launch(std::integral_constant<int, 8>{});
         }
         if (waves >= 4) {
@@ -142,6 +156,27 @@ extern "C" int kush_append_decode(int head_dim, int bits, int group, int dtype, 
     return decode_impl("kush_append_decode", head_dim, bits, group, dtype, q, out, cache, block_stride, head_stride,
                        tail_k, tail_idx, block_table, seq_lens, bt_stride, bt_cols, hkv, scale, n_splits, part_ml, part_o,
                        split_sync, waves, seq_order, n_seqs, rot, Append{k, v, k_row_stride, v_row_stride}, stream);
+}
+
+extern "C" int kush_window_decode(int head_dim, int bits, int group, int dtype, const void* q, void* out, void* cache,
+                                  int64_t block_stride, int64_t head_stride, void* tail_k, const int32_t* tail_idx,
+                                  const int32_t* block_table, const int32_t* seq_lens, int64_t bt_stride, int32_t hkv,
+                                  float scale, int32_t n_splits, float* part_ml, float* part_o, int32_t n_seqs,
+                                  void* stream, const void* k, const void* v, int64_t k_row_stride,
+                                  int64_t v_row_stride, int32_t* split_sync, int32_t waves, const int32_t* seq_order,
+                                  int32_t rot, int32_t window, int32_t sinks) {
+    if (window <= 0 || sinks < 0) return kush_fail(-2, "kush_window_decode: bad window %d / sinks %d", window, sinks);
+    if ((k == nullptr) != (v == nullptr)) return kush_fail(-2, "kush_window_decode: k and v go together");
+    if (k != nullptr && group > 16)
+        return kush_fail(-2, "kush_window_decode: group %d > 16 (append first: k and v null)", group);
+    const int64_t e = dtype == 0 ? 4 : 2;
+    if (k != nullptr &&
+        (((uintptr_t)k | (uintptr_t)v | (uint64_t)(k_row_stride * e) | (uint64_t)(v_row_stride * e)) & 15))
+        return kush_fail(-2, "kush_window_decode: k / v rows must be 16-byte aligned (append first: k and v null)");
+    return decode_impl("kush_window_decode", head_dim, bits, group, dtype, q, out, cache, block_stride, head_stride, tail_k,
+                       tail_idx, block_table, seq_lens, bt_stride, 0, hkv, scale, n_splits, part_ml, part_o, split_sync,
+                       waves, seq_order, n_seqs, rot, Append{k, v, k_row_stride, v_row_stride}, stream,
+                       Window{window, sinks});
 }
 
 extern "C" int kush_combine_ex(int head_dim, int group, int dtype, void* out, const float* part_ml, const float* part_o,
