@@ -46,10 +46,13 @@ int kush_step_maps(const int32_t* new_tokens, const int32_t* history, const int3
  *   min_p > 0    of those, the tokens with w >= min_p
  * the first token always. out[r] is the first index whose running sum of kept w, in the vocabulary's order, exceeds
  * uniforms[r] times the sum of all. temperature 0: the first of the order. A row with a NaN, or with no logit above
- * -inf: -1. The parameters are one value for all rows, or (pointer not null) one per row. */
+ * -inf: -1. The parameters are one value for all rows, or (pointer not null) one per row. scratch: kush_sample_scratch(rows,
+ * vocab) bytes, 16-byte aligned, of any contents, this call's own until it has run. */
+int64_t kush_sample_scratch(int64_t rows, int64_t vocab);
 int kush_sample(int dtype, const void* logits, int64_t row_stride, int64_t rows, int64_t vocab, const float* uniforms,
                 double temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks, double top_p,
-                const float* top_ps, double min_p, const float* min_ps, int64_t* out, void* stream);
+                const float* top_ps, double min_p, const float* min_ps, int64_t* out, void* scratch, int64_t scratch_bytes,
+                void* stream);
 
 #ifdef __cplusplus
 }

@@ -80,8 +80,10 @@ STEP_SIGNATURES = {
     # new_tokens, history, slots, block_table, bt_row_stride, bt_cols, n_reqs, window, sinks, jobs, pages, tails, tokens,
     # the eleven outputs, stream
     "kush_step_maps": [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I64, _I64, _I64, _I64] + [_P] * 12,
-    # dtype, logits, row_stride, rows, vocab, uniforms, then (value, per row) of temperature, top_k, top_p, min_p; out, stream
-    "kush_sample": [_I32, _P, _I64, _I64, _I64, _P, _F64, _P, _I32, _P, _F64, _P, _F64, _P, _P, _P],
+    # dtype, logits, row_stride, rows, vocab, uniforms, then (value, per row) of temperature, top_k, top_p, min_p; out, scratch,
+    # scratch_bytes, stream
+    "kush_sample": [_I32, _P, _I64, _I64, _I64, _P, _F64, _P, _I32, _P, _F64, _P, _F64, _P, _P, _P, _I64, _P],
+    "kush_sample_scratch": [_I64, _I64],                         # returns bytes
 }
 
 
@@ -97,7 +99,7 @@ def lib() -> ctypes.CDLL:
     for name, args in (SIGNATURES | ATTEND_SIGNATURES | WINDOW_SIGNATURES | STEP_SIGNATURES).items():
         fn = getattr(cdll, name)
         fn.argtypes = args
-        fn.restype = ctypes.c_char_p if name == "kush_last_error" else ctypes.c_int32
+        fn.restype = {"kush_last_error": ctypes.c_char_p, "kush_sample_scratch": _I64}.get(name, ctypes.c_int32)
     return cdll
 
 

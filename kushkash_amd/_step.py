@@ -237,6 +237,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         out = torch.empty(B, dtype=torch.int64, device=dev)
     _index("out", out, B, dev, (torch.int64,))
     if B:
+        from . import _lib
+        scratch = torch.empty(_lib.lib().kush_sample_scratch(B, V), dtype=torch.uint8, device=dev)
         _call("kush_sample", dev, _CODE[logits.dtype], logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V,
-              uniforms.data_ptr(), *settings, out.data_ptr())
+              uniforms.data_ptr(), *settings, out.data_ptr(), scratch.data_ptr(), scratch.numel())
     return out

@@ -126,334 +126,589 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------ sampling
+// One token per row in four launches; every sum is an integer, so no order of workgroups, lanes or atomics changes it.
+// A weight w = exp((x - max) / T) is held as a multiple of 2^-bits in 64 bits (bits such that the vocabulary's sum fits),
+// off by 2^-bits-1: far below what a 24-bit random number resolves.
+//   1. sample_max     every workgroup a piece of a row: its largest logit and where, its smallest, NaN; the row's bins
+//                     cleared for the next launch
+//   2. sample_bins    the tokens in BINS classes of equal width below the largest logit (class 0: next to it), their
+//                     number and, where top-p asks, their mass: in LDS, the classes that are not empty added to the row's
+//   3. sample_pick    the classes that the cuts of top-k and top-p fall into, from the bins; the mass of every tile's
+//                     tokens above them; the tokens inside them to the row's list (a few hundred of 150,000, as a rule)
+//   4. sample_token   the list sorted: the exact cuts, ties by index; the tile that u times the kept mass falls into,
+//                     and the token in it
+// A list of more than LIST tokens (thousands of equal logits next to a cut) is cut by a radix search over the row instead.
 struct SampleArgs {
     const void* logits;
     int64_t stride;
-    int vocab, bits;                 // weights are held as multiples of 2^-bits
+    int vocab, bits, tiles, per;     // tiles of TILE tokens, `per` of them to a workgroup
     const float* uniforms;
     double temperature, top_p, min_p;
     int top_k;
     const float *temperatures, *top_ps, *min_ps;
     const int32_t* top_ks;
     int64_t* out;
+    // scratch, per row: parts [pieces], bins [BINS] mass and count, tile sums [tiles], the list's length, the list
+    struct SamplePart* parts;
+    uint64_t *mass, *sums;
+    uint32_t *count, *length;
+    uint2* list;
+    int64_t row0;                    // the first row of this launch (its scratch is row 0's)
 };
 
-constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / WAVE;
-constexpr int BINS = 2048;           // of a radix pass: 11, 11 and 10 bits of a logit's order
+// A piece of a row
+struct SamplePart {
+    float most, least;               // least: the smallest above -inf
+    int at;                          // the first index of most
+    int nan;
+};
+
+constexpr int BINS = 1024, TILE = 4096, LIST = 8192, PIECE_THREADS = 256;
+constexpr float SPAN = 64.0f;        // logits (in units of max(1, T)) that the bins cover at most
 
 // logits in an order of their own: larger logit, larger key; -0 and 0 alike
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 
-// E elements of T from p, whatever its alignment
-template <typename T, int E>
-__device__ __forceinline__ void load_elems(const T* p, float (&x)[E]) {
-    T v[E];
-    __builtin_memcpy(v, p, sizeof(v));
+// 2^t for t <= 0: e^z, |z| <= ln 2 / 2, by its Taylor polynomial of degree 12 (2e-16 off), times a power of two
+__device__ __forceinline__ double exp2_64(double t) {
+    const double n = __builtin_rint(t), z = (t - n) * 0.693147180559945309417;       // 2^f = e^z
+    double p = 0.0;
+    constexpr double inv[13] = {1.0,          1.0,           1.0 / 2,        1.0 / 6,          1.0 / 24,
+                                1.0 / 120,    1.0 / 720,     1.0 / 5040,     1.0 / 40320,      1.0 / 362880,
+                                1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = to_f32(v[e]);
+    for (int i = 12; i >= 0; --i) p = __builtin_fma(p, z, inv[i]);
+    return t < -1100.0 ? 0.0 : __builtin_ldexp(p, (int)n);
 }
 
-// What a row's tokens are kept by: those above key, and of those at key the first `ties` by index
-struct Cut {
-    uint32_t key;
-    int ties;
+// What a row is drawn with, and where its weights and bins are counted from
+struct SampleRow {
+    double c, top_p, min_p;          // c = log2 e / T
+    float most, scale;               // scale: bins per logit
+    int top_k, at;                   // top_k 0: off; at: the first of the order
+    bool none, greedy, by_mass;
+    int bits;
+    __device__ __forceinline__ double weight(float x) const { return exp2_64(x == most ? 0.0 : ((double)x - (double)most) * c); }
+    // w >= 0 in multiples of 2^-bits, at least one where w is above 0
+    __device__ __forceinline__ uint64_t fixed(double w) const {
+        const double big = __builtin_fma(w, __builtin_ldexp(1.0, bits), 4503599627370496.0);       // + 2^52
+        const uint64_t m = __builtin_bit_cast(uint64_t, big) & 0xFFFFFFFFFFFFFull;
+        return w > 0.0 ? (m ? m : 1) : 0;
+    }
+    // the class of a logit: as d = most - x grows, never smaller
+    __device__ __forceinline__ int bin(float x) const {
+        const float d = x == most ? 0.0f : (most - x) * scale;
+        return d < (float)(BINS - 1) ? (int)d : BINS - 1;
+    }
 };
 
+// x is 16 bytes of a row's logits; elements past the vocabulary read as -inf
 template <typename T>
-struct Sampler {
-    static constexpr int E = 16 / sizeof(T), TILE = SAMPLE_THREADS * E;
-    const T* row;
-    int vocab, tid, lane, w;
-    float most;
-    double inv_t;
-    int bits;
-
-    // fn(index, value) of every logit, index ascending within a thread; a wave's lanes take adjacent runs of E
-    template <typename Fn>
-    __device__ __forceinline__ void each(Fn&& fn) const {
-        for (int i0 = tid * E; i0 < vocab; i0 += TILE) {
-            float x[E];
-            if (i0 + E <= vocab) {
-                load_elems<T, E>(row + i0, x);
+struct Chunk {
+    static constexpr int E = 16 / sizeof(T);
+    float x[E];
+    __device__ __forceinline__ void load(const T* row, int i, int vocab) {
+        if (i + E <= vocab) {
+            T v[E];
+            __builtin_memcpy(v, row + i, sizeof(v));
 #pragma unroll
-                for (int e = 0; e < E; ++e) fn(i0 + e, x[e]);
-            } else {
-                for (int i = i0; i < vocab; ++i) fn(i, to_f32(row[i]));
-            }
+            for (int e = 0; e < E; ++e) x[e] = to_f32(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = i + e < vocab ? to_f32(row[i + e]) : -__builtin_inff();
         }
     }
-    // w in multiples of 2^-bits; at least 1 of them where w is above 0
-    __device__ __forceinline__ uint64_t weight(float x, double& wd) const {
-        wd = x == most ? 1.0 : exp(((double)x - (double)most) * inv_t);
-        return wd > 0.0 ? max((uint64_t)1, (uint64_t)(wd * (double)(1ull << bits) + 0.5)) : 0;
-    }
 };
 
-template <typename X>
-__device__ __forceinline__ X block_sum(X x, X* part, int lane, int w) {
+// fn(index of the first, chunk) over this thread's chunks of a tile
+template <typename T, int THREADS, typename Fn>
+__device__ __forceinline__ void tile_chunks(const T* row, int tile, int vocab, Fn&& fn) {
+    constexpr int E = Chunk<T>::E, N = TILE / (THREADS * E);
+    static_assert(N * THREADS * E == TILE, "whole chunks");
+    Chunk<T> c[N];
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, WAVE);
+    for (int j = 0; j < N; ++j) c[j].load(row, tile * TILE + (j * THREADS + (int)threadIdx.x) * E, vocab);
+#pragma unroll
+    for (int j = 0; j < N; ++j) fn(tile * TILE + (j * THREADS + (int)threadIdx.x) * E, c[j]);
+}
+
+__device__ __forceinline__ SamplePart merge_parts(SamplePart a, const SamplePart& b) {
+    if (b.most > a.most || (b.most == a.most && b.at < a.at)) {
+        a.most = b.most;
+        a.at = b.at;
+    }
+    a.least = __builtin_fminf(a.least, b.least);
+    a.nan |= b.nan;
+    return a;
+}
+__device__ __forceinline__ SamplePart wave_part(SamplePart p) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1)
+        p = merge_parts(p, SamplePart{__shfl_xor(p.most, m, WAVE), __shfl_xor(p.least, m, WAVE), __shfl_xor(p.at, m, WAVE),
+                                      __shfl_xor(p.nan, m, WAVE)});
+    return p;
+}
+constexpr SamplePart NO_PART{-__builtin_inff(), __builtin_inff(), 0x7fffffff, 0};
+
+template <typename T>
+__global__ __launch_bounds__(PIECE_THREADS) void sample_max(const SampleArgs a) {
+    __shared__ SamplePart ws[PIECE_THREADS / WAVE];
+    const int64_t s = blockIdx.y, r = a.row0 + s;
+    const int piece = blockIdx.x, pieces = gridDim.x, tid = threadIdx.x;
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    for (int i = piece * PIECE_THREADS + tid; i < BINS; i += pieces * PIECE_THREADS) {
+        a.mass[s * BINS + i] = 0;
+        a.count[s * BINS + i] = 0;
+    }
+    if (piece == 0 && tid == 0) a.length[s] = 0;
+    SamplePart p = NO_PART;
+    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t)
+        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
+#pragma unroll
+            for (int e = 0; e < Chunk<T>::E; ++e) {
+                const float x = c.x[e];
+                p.nan |= x != x;
+                p.least = x > -__builtin_inff() ? __builtin_fminf(p.least, x) : p.least;
+                if (x > p.most) {
+                    p.most = x;
+                    p.at = i + e;
+                }
+            }
+        });
+    p = wave_part(p);
+    if (tid % WAVE == 0) ws[tid / WAVE] = p;
     __syncthreads();
-    if (lane == 0) part[w] = x;
-    __syncthreads();
-    x = part[0];
-    for (int i = 1; i < SAMPLE_WAVES; ++i) x += part[i];
+    if (tid == 0) {
+        for (int w = 1; w < PIECE_THREADS / WAVE; ++w) p = merge_parts(p, ws[w]);
+        a.parts[s * pieces + piece] = p;
+    }
+}
+
+// A row's settings and its parts put together, by every wave for itself (the same in all lanes)
+__device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, int pieces) {
+    const int64_t r = a.row0 + s;
+    SamplePart p = NO_PART;
+    for (int i = threadIdx.x % WAVE; i < pieces; i += WAVE) p = merge_parts(p, a.parts[s * pieces + i]);
+    p = wave_part(p);
+    const double temp = a.temperatures ? (double)a.temperatures[r] : a.temperature;
+    SampleRow x;
+    x.top_p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
+    x.min_p = a.min_ps ? (double)a.min_ps[r] : a.min_p;
+    const int k = a.top_ks ? a.top_ks[r] : a.top_k;
+    x.top_k = k > 0 && k < a.vocab ? k : 0;
+    x.by_mass = x.top_p < 1.0;
+    x.none = p.nan || p.most == -__builtin_inff();
+    x.greedy = !(temp > 0.0);
+    x.most = p.most;
+    x.at = p.at;
+    x.bits = a.bits;
+    x.c = 1.44269504088896340736 / temp;
+    // the row's own span, so that a flat row has bins as well, but no more than what matters: SPAN logits for a count,
+    // SPAN temperatures for a mass alone
+    const float unit = x.top_k ? __builtin_fmaxf(1.0f, (float)temp) : (float)temp;
+    const float span = __builtin_fminf(p.most - p.least, SPAN * unit);
+    x.scale = span > 0.0f && span < __builtin_inff() ? __builtin_fminf((BINS - 1) / span, 1e30f) : 1.0f;
     return x;
 }
 
-// grid rows, block 1024: one row. The weights are held as 64-bit multiples of 2^-bits (bits such that their sum over the
-// vocabulary fits): sums are exact, so no order of atomics or lanes changes a token, and each weight is off by 2^-bits-1,
-// far below what a 24-bit random number resolves.
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(PIECE_THREADS) void sample_bins(const SampleArgs a) {
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
-    __shared__ uint64_t part[SAMPLE_WAVES];
-    __shared__ uint64_t found_mass;
-    __shared__ int found_bin, found_count;
-    Sampler<T> s;
-    const int64_t r = blockIdx.x;
-    s.row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
-    s.vocab = a.vocab;
-    s.tid = threadIdx.x;
-    s.lane = s.tid % WAVE;
-    s.w = s.tid / WAVE;
-    s.bits = a.bits;
-    const double temp = a.temperatures ? (double)a.temperatures[r] : a.temperature;
-    const double top_p = a.top_ps ? (double)a.top_ps[r] : a.top_p, min_p = a.min_ps ? (double)a.min_ps[r] : a.min_p;
-    const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-
-    // the largest logit and its first index; NaN
-    float mx = -__builtin_inff();
-    int at = 0x7fffffff, bad = 0;
-    s.each([&](int i, float x) {
-        bad |= x != x;
-        if (x > mx) {
-            mx = x;
-            at = i;
-        }
-    });
+    const int64_t s = blockIdx.y, r = a.row0 + s;
+    const int piece = blockIdx.x, tid = threadIdx.x;
+    const SampleRow x = sample_row(a, s, gridDim.x);
+    if (x.none || x.greedy || (!x.top_k && !x.by_mass)) return;
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    for (int i = tid; i < BINS; i += PIECE_THREADS) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
+    __syncthreads();
+    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t)
+        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        const float ox = __shfl_xor(mx, m, WAVE);
-        const int oi = __shfl_xor(at, m, WAVE);
-        bad |= __shfl_xor(bad, m, WAVE);
-        if (ox > mx || (ox == mx && oi < at)) {
-            mx = ox;
-            at = oi;
-        }
-    }
-    if (s.lane == 0) {
-        mass[s.w] = ((uint64_t)order_key(mx) << 32) | (uint32_t)~at;
-        count[s.w] = bad;
-    }
-    __syncthreads();
-    uint64_t best = 0;
-    for (int i = 0; i < SAMPLE_WAVES; ++i) {
-        best = max(best, mass[i]);
-        bad |= count[i];
-    }
-    at = (int)~(uint32_t)best;
-    const uint32_t top_key = (uint32_t)(best >> 32);
-    s.most = __uint_as_float(top_key ^ ((top_key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-    __syncthreads();
-    if (bad || s.most == -__builtin_inff()) {
-        if (s.tid == 0) a.out[r] = -1;
-        return;
-    }
-    if (!(temp > 0.0)) {
-        if (s.tid == 0) a.out[r] = at;
-        return;
-    }
-    s.inv_t = 1.0 / temp;
-
-    // The cut after the first `want` tokens (by_mass: after the tokens with less than `limit` mass before them) of what
-    // `cut` keeps: a radix search over the keys, 11 bits a pass. before: the mass above the bins searched.
-    const auto narrow = [&](Cut cut, bool by_mass, int want, double limit, uint64_t& kept_mass) -> Cut {
-        uint32_t prefix = 0;
-        uint64_t above_mass = 0;
-        int above = 0;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), nb = pass == 2 ? 1024 : 2048;
-            for (int i = s.tid; i < BINS; i += SAMPLE_THREADS) {
-                mass[i] = 0;
-                count[i] = 0;
-            }
-            __syncthreads();
-            s.each([&](int, float x) {
-                const uint32_t k = order_key(x);
-                if (k < cut.key || (pass > 0 && (k >> (shift + (pass == 1 ? 11 : 10))) != prefix)) return;
-                double wd;
-                const uint32_t b = (k >> shift) & (nb - 1);
+            for (int e = 0; e < Chunk<T>::E; ++e) {
+                if (i + e >= a.vocab) continue;
+                const int b = x.bin(c.x[e]);
                 atomicAdd(&count[b], 1u);
-                atomicAdd((unsigned long long*)&mass[b], (unsigned long long)s.weight(x, wd));
-            });
-            __syncthreads();
-            // the bins from the top: each thread's two, then a scan over the threads (2 bins each, the highest first)
-            const int b1 = nb - 1 - 2 * s.tid, b0 = b1 - 1;
-            const bool live = b0 >= 0;
-            uint32_t c1 = live ? count[b1] : 0, c0 = live ? count[b0] : 0;
-            uint64_t m1 = live ? mass[b1] : 0, m0 = live ? mass[b0] : 0;
-            // tokens at cut.key count as far as the cut keeps them (all of one key: the last pass's bin)
-            uint64_t cs = c1 + c0, ms = m1 + m0;
-            for (int d = 1; d < WAVE; d <<= 1) {
-                const uint64_t oc = __shfl_up(cs, d, WAVE), om = __shfl_up(ms, d, WAVE);
-                if (s.lane >= d) {
-                    cs += oc;
-                    ms += om;
-                }
+                if (x.by_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(c.x[e])));
             }
-            __syncthreads();
-            if (s.lane == WAVE - 1) part[s.w] = ms;
-            __syncthreads();
-            uint64_t base_m = 0;
-            for (int i = 0; i < s.w; ++i) base_m += part[i];
-            __syncthreads();
-            if (s.lane == WAVE - 1) part[s.w] = cs;
-            if (s.tid == 0) found_bin = -1;
-            __syncthreads();
-            uint64_t base_c = 0;
-            for (int i = 0; i < s.w; ++i) base_c += part[i];
-            // the first bin behind which the cut lies
-            uint64_t cb = above + base_c + cs - c1 - c0, mb = above_mass + base_m + ms - m1 - m0;
-            if (live) {
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t c = j == 0 ? c1 : c0;
-                    const uint64_t m = j == 0 ? m1 : m0;
-                    const bool here = by_mass ? (double)mb < limit && !((double)(mb + m) < limit) : cb < (uint64_t)want && cb + c >= (uint64_t)want;
-                    if (here && c > 0) {
-                        found_bin = j == 0 ? b1 : b0;
-                        found_mass = mb;
-                        found_count = (int)cb;
-                    }
-                    cb += c;
-                    mb += m;
-                }
-            }
-            __syncthreads();
-            if (found_bin < 0) return cut;                               // everything is kept
-            above = found_count;
-            above_mass = found_mass;
-            prefix = pass == 0 ? found_bin : ((prefix << (pass == 1 ? 11 : 10)) | found_bin);
-            __syncthreads();
-        }
-        // all of one key: equal weights
-        double wd;
-        const uint32_t kb = prefix ^ ((prefix >> 31) ? 0x80000000u : 0xFFFFFFFFu);
-        const uint64_t each = s.weight(__uint_as_float(kb), wd);
-        int ties;
-        if (by_mass) {
-            const double left = (limit - (double)above_mass) / (double)max(each, (uint64_t)1);
-            ties = (int)fmin(ceil(left), 2147483647.0);
-        } else {
-            ties = want - above;
-        }
-        if (prefix == cut.key) ties = min(ties, cut.ties);
-        kept_mass = above_mass + each * (uint64_t)ties;
-        return Cut{prefix, max(ties, 1)};
-    };
-
-    Cut cut{0, 0x7fffffff};
-    if (top_k > 0 || top_p < 1.0) {
-        uint64_t total = 0;
-        s.each([&](int, float x) {
-            double wd;
-            total += s.weight(x, wd);
         });
-        total = block_sum(total, part, s.lane, s.w);
-        if (top_k > 0 && top_k < s.vocab) cut = narrow(cut, false, top_k, 0.0, total);
-        if (top_p < 1.0) {
-            uint64_t unused = 0;
-            cut = narrow(cut, true, 0, fmax(top_p * (double)total, 0.5), unused);
+    __syncthreads();
+    for (int i = tid; i < BINS; i += PIECE_THREADS)
+        if (count[i]) {
+            atomicAdd(&a.count[s * BINS + i], count[i]);
+            if (x.by_mass) atomicAdd((unsigned long long*)&a.mass[s * BINS + i], (unsigned long long)mass[i]);
+        }
+}
+
+template <int THREADS, typename X>
+__device__ __forceinline__ X block_scan(X x, X* part, X& all) {             // inclusive, in thread order
+    const int lane = threadIdx.x % WAVE, w = threadIdx.x / WAVE;
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) {
+        const X o = __shfl_up(x, d, WAVE);
+        if (lane >= d) x += o;
+    }
+    __syncthreads();
+    if (lane == WAVE - 1) part[w] = x;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / WAVE; ++i) {
+        if (i < w) x += part[i];
+        all += part[i];
+    }
+    return x;
+}
+
+// The classes that the cuts fall into: everything below lo is kept (after the other cuts), lo .. hi and k are looked at
+// token by token, all else is dropped. before_lo, before_k: mass below those classes; above_k: tokens below k.
+struct SampleCuts {
+    int lo, hi, k;
+    uint64_t before_lo, before_k;
+    uint32_t above_k;
+};
+
+// top-p's limit for a mass of `total` (at least half a unit: the first token is kept)
+__device__ __forceinline__ double mass_limit(const SampleRow& x, uint64_t total) {
+    return __builtin_fmax(x.top_p * (double)total, 0.5);
+}
+
+template <int THREADS>
+__device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64_t s) {
+    __shared__ uint64_t part[THREADS / WAVE];
+    __shared__ SampleCuts cuts;
+    constexpr int N = BINS / THREADS;
+    const int tid = threadIdx.x;
+    uint32_t c[N];
+    uint64_t m[N], cs = 0, ms = 0, c_all, m_all;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        c[i] = a.count[s * BINS + tid * N + i];
+        m[i] = x.by_mass ? a.mass[s * BINS + tid * N + i] : 0;
+        cs += c[i];
+        ms += m[i];
+    }
+    if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0};
+    const uint64_t c1 = block_scan<THREADS>(cs, part, c_all), m1 = block_scan<THREADS>(ms, part, m_all);
+    if (x.top_k) {
+        uint64_t cb = c1 - cs, mb = m1 - ms;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (cb < (uint64_t)x.top_k && cb + c[i] >= (uint64_t)x.top_k) {
+                cuts.k = tid * N + i;
+                cuts.above_k = (uint32_t)cb;
+                cuts.before_k = mb;
+            }
+            cb += c[i];
+            mb += m[i];
         }
     }
-
-    // The running sum in index order: tiles in turn, each wave's kept mass and ties of a tile, the tile that the target
-    // falls into, the wave, the lane. Two rounds: the sum of all, then the search.
-    const auto tile_mass = [&](int i0, int& tie_base, uint64_t (&wt)[Sampler<T>::E]) -> uint64_t {
-        constexpr int E = Sampler<T>::E;
-        uint64_t sum = 0;
-        int ties = 0;
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = i0 + e < s.vocab ? to_f32(s.row[i0 + e]) : -__builtin_inff();
-            ties += i0 + e < s.vocab && order_key(x[e]) == cut.key;
-        }
-        // ties before this lane's in the tile
-        int scan = ties;
-        for (int d = 1; d < WAVE; d <<= 1) {
-            const int o = __shfl_up(scan, d, WAVE);
-            if (s.lane >= d) scan += o;
-        }
-        __syncthreads();
-        if (s.lane == WAVE - 1) count[s.w] = scan;
-        __syncthreads();
-        int base = tie_base, all = 0;
-        for (int i = 0; i < SAMPLE_WAVES; ++i) {
-            if (i < s.w) base += count[i];
-            all += count[i];
-        }
-        base += scan - ties;
-        tie_base += all;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            wt[e] = 0;
-            if (i0 + e >= s.vocab) continue;
-            const uint32_t k = order_key(x[e]);
-            double wd;
-            const uint64_t m = s.weight(x[e], wd);
-            const bool kept = (k > cut.key || (k == cut.key && base++ < cut.ties)) && (wd >= min_p || i0 + e == at);
-            wt[e] = kept ? m : 0;
-            sum += wt[e];
-        }
-        return sum;
-    };
-    uint64_t mine = 0;
-    int tie_base = 0;
-    uint64_t wt[Sampler<T>::E];
-    for (int t0 = 0; t0 < s.vocab; t0 += Sampler<T>::TILE) mine += tile_mass(t0 + s.tid * Sampler<T>::E, tie_base, wt);
-    const uint64_t all = block_sum(mine, part, s.lane, s.w);
-    const float u = a.uniforms[r];
-    // the largest target is the last kept token's
-    const double want = fmin((double)fmaxf(u, 0.0f) * (double)all, (double)(all - 1));
-    uint64_t run = 0;
-    tie_base = 0;
-    if (s.tid == 0) found_bin = -1;
     __syncthreads();
-    for (int t0 = 0; t0 < s.vocab; t0 += Sampler<T>::TILE) {
-        const int i0 = t0 + s.tid * Sampler<T>::E;
-        const uint64_t sum = tile_mass(i0, tie_base, wt);
-        uint64_t scan = sum;
-        for (int d = 1; d < WAVE; d <<= 1) {
-            const uint64_t o = __shfl_up(scan, d, WAVE);
-            if (s.lane >= d) scan += o;
+    const SampleCuts now = cuts;
+    __syncthreads();
+    if (!x.by_mass) {
+        if (tid == 0) cuts.lo = cuts.hi = now.k;
+    } else {
+        // the kept mass lies between what is below k and what k adds: so does top-p's cut
+        uint64_t mb = m1 - ms;
+        const double low = mass_limit(x, x.top_k ? now.before_k : m_all);
+        double high = low;
+        if (x.top_k) high = mass_limit(x, now.before_k + a.mass[s * BINS + now.k]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint64_t me = mb + m[i];
+            if ((double)mb < low && !((double)me < low)) {
+                cuts.lo = tid * N + i;
+                cuts.before_lo = mb;
+            }
+            if ((double)mb < high && !((double)me < high)) cuts.hi = tid * N + i;
+            mb = me;
         }
-        if (s.lane == WAVE - 1) part[s.w] = scan;
-        __syncthreads();
-        uint64_t before = run, tile = 0;
-        for (int i = 0; i < SAMPLE_WAVES; ++i) {
-            if (i < s.w) before += part[i];
-            tile += part[i];
-        }
-        before += scan - sum;
-        if ((double)before <= want && (double)(before + sum) > want && sum > 0) {
-            for (int e = 0; e < Sampler<T>::E; ++e) {
-                before += wt[e];
-                if ((double)before > want) {
-                    found_bin = i0 + e;
-                    break;
+    }
+    __syncthreads();
+    return cuts;
+}
+
+template <typename T>
+__global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a) {
+    __shared__ unsigned long long sum;
+    const int64_t s = blockIdx.y, r = a.row0 + s;
+    const int piece = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE;
+    const SampleRow x = sample_row(a, s, gridDim.x);
+    if (x.none || x.greedy) return;
+    SampleCuts cut{BINS, BINS, BINS, 0, 0, 0};
+    if (x.top_k || x.by_mass) cut = sample_cuts<PIECE_THREADS>(a, x, s);
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t) {
+        uint64_t mine = 0;
+        if (tid == 0) sum = 0;
+        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
+#pragma unroll
+            for (int e = 0; e < Chunk<T>::E; ++e) {
+                const int b = x.bin(c.x[e]);
+                const bool real = i + e < a.vocab;
+                if (real && b < cut.lo) {
+                    const double w = x.weight(c.x[e]);
+                    if (w >= x.min_p || i + e == x.at) mine += x.fixed(w);
+                }
+                const bool look = real && b >= cut.lo && (b <= cut.hi || b == cut.k);
+                const uint64_t who = __ballot(look);
+                if (who) {                                            // the wave's tokens, side by side
+                    uint32_t at = 0;
+                    const int leader = __builtin_ctzll(who);
+                    if (lane == leader) at = atomicAdd(&a.length[s], (uint32_t)__popcll(who));
+                    at = __shfl(at, leader, WAVE) + __popcll(who & ((1ull << lane) - 1));
+                    if (look && at < LIST) a.list[s * LIST + at] = uint2{(uint32_t)(i + e), order_key(c.x[e])};
                 }
             }
-        }
-        run += tile;
+        });
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) mine += __shfl_xor(mine, m, WAVE);
         __syncthreads();
-        if (found_bin >= 0) break;
+        if (lane == 0 && mine) atomicAdd(&sum, (unsigned long long)mine);
+        __syncthreads();
+        if (tid == 0) a.sums[s * a.tiles + t] = sum;
+        __syncthreads();
     }
-    if (s.tid == 0) a.out[r] = found_bin >= 0 ? found_bin : at;
+}
+
+constexpr int TOKEN_THREADS = 1024, MAX_TILES = (1 << 24) / TILE;
+
+// The order as one number, larger first: the key, then the smaller index
+__device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
+
+// grid rows. What is kept of the row: tokens of classes below `lo`, and those of order `least` or above; w >= min_p.
+template <typename T>
+__global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a, int pieces) {
+    __shared__ uint64_t list[LIST];
+    __shared__ unsigned long long sums[MAX_TILES];
+    __shared__ uint64_t part[TOKEN_THREADS / WAVE];
+    __shared__ uint64_t shared_mass;
+    __shared__ int shared_at;
+    const int64_t s = blockIdx.x, r = a.row0 + s;
+    const int tid = threadIdx.x;
+    const SampleRow x = sample_row(a, s, pieces);
+    if (x.none || x.greedy) {
+        if (tid == 0) a.out[r] = x.none ? -1 : x.at;
+        return;
+    }
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    int lo = BINS;                                       // all is kept
+    uint64_t least = ~0ull;
+    const int n = x.top_k || x.by_mass ? (int)min(a.length[s], (uint32_t)0x7fffffff) : 0;
+    for (int i = tid; i < a.tiles; i += TOKEN_THREADS) sums[i] = a.sums[s * a.tiles + i];
+    if (x.top_k || x.by_mass) {
+        const SampleCuts cut = sample_cuts<TOKEN_THREADS>(a, x, s);
+        lo = cut.lo;
+        if (n <= LIST) {
+            // sorted, the largest first (bitonic; the places behind the list hold 0, below every token)
+            int size = 2;
+            while (size < n) size <<= 1;
+            for (int i = tid; i < size; i += TOKEN_THREADS)
+                list[i] = i < n ? order_of(a.list[s * LIST + i].y, a.list[s * LIST + i].x) : 0;
+            __syncthreads();
+            for (int k = 2; k <= size; k <<= 1)
+                for (int j = k >> 1; j > 0; j >>= 1) {
+                    for (int i = tid; i < size / 2; i += TOKEN_THREADS) {
+                        const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1)), q = p | j;
+                        const uint64_t u = list[p], v = list[q];
+                        if ((u < v) == ((p & k) == 0)) {
+                            list[p] = v;
+                            list[q] = u;
+                        }
+                    }
+                    __syncthreads();
+                }
+            // each thread a run of the sorted list; weights in registers
+            const int run = (size + TOKEN_THREADS - 1) / TOKEN_THREADS;          // LIST / TOKEN_THREADS at most
+            uint64_t m[LIST / TOKEN_THREADS], mine = 0, in_k = 0;
+            const auto token = [&](int i) { return key_logit((uint32_t)(list[i] >> 32)); };
+            // of class k, the first top_k - above_k tokens: their mass makes the kept mass exact
+            int k_first = n;
+            if (x.top_k) {
+                if (tid == 0) shared_at = n;
+                __syncthreads();
+                for (int i = tid; i < n; i += TOKEN_THREADS)
+                    if (x.bin(token(i)) == cut.k && (i == 0 || x.bin(token(i - 1)) != cut.k)) shared_at = i;
+                __syncthreads();
+                k_first = shared_at;
+            }
+            const int k_end = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : n;     // the list's tokens up to top-k's cut
+#pragma unroll
+            for (int e = 0; e < LIST / TOKEN_THREADS; ++e) {
+                const int i = tid * run + e;
+                m[e] = e < run && i < n && x.by_mass ? x.fixed(x.weight(token(i))) : 0;
+                mine += m[e];
+                if (i >= k_first && i < k_end) in_k += m[e];
+            }
+            int keep = k_end;
+            if (x.by_mass) {
+                uint64_t all, k_mass;
+                uint64_t before = block_scan<TOKEN_THREADS>(mine, part, all) - mine + cut.before_lo;
+                block_scan<TOKEN_THREADS>(in_k, part, k_mass);
+                uint64_t total = cut.before_k + k_mass;
+                if (!x.top_k) {                                    // the mass of the row
+                    uint64_t sum = 0;
+                    for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
+                    block_scan<TOKEN_THREADS>(sum, part, total);
+                }
+                const double limit = mass_limit(x, total);
+                int here = 0;
+#pragma unroll
+                for (int e = 0; e < LIST / TOKEN_THREADS; ++e) {
+                    const int i = tid * run + e;
+                    if (e < run && i < n) here += (double)before < limit;
+                    before += m[e];
+                }
+                int kept_all;
+                block_scan<TOKEN_THREADS>(here, reinterpret_cast<int*>(part), kept_all);
+                keep = min(keep, kept_all);
+            }
+            least = keep > 0 ? list[keep - 1] : ~0ull;
+            // the kept tokens' mass to their tiles
+            __syncthreads();
+            for (int i = tid; i < keep; i += TOKEN_THREADS) {
+                const double w = x.weight(token(i));
+                const uint32_t at = ~(uint32_t)list[i];
+                if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)x.fixed(w));
+            }
+        } else {
+            // the token that ends what is kept, by a radix search over the row's orders: 11 bits a pass, from the top
+            uint64_t* const mass = list;
+            uint32_t* const count = reinterpret_cast<uint32_t*>(list + 2048);
+            const auto each = [&](auto&& fn) {
+                for (int i = tid; i < a.vocab; i += TOKEN_THREADS) fn(i, to_f32(row[i]));
+            };
+            // of the tokens of order `floor` and above: the `want`-th, or the last with less than `limit` mass before it;
+            // kept: the mass up to it
+            const auto search = [&](bool by_mass, uint64_t floor, uint32_t want, double limit, uint64_t& kept) -> uint64_t {
+                uint64_t prefix = 0, above_mass = 0, above = 0;
+                for (int top = 64; top > 0;) {
+                    const int width = min(11, top), shift = top - width, nb = 1 << width;
+                    __syncthreads();
+                    for (int i = tid; i < 2048; i += TOKEN_THREADS) {
+                        mass[i] = 0;
+                        count[i] = 0;
+                    }
+                    __syncthreads();
+                    each([&](int i, float v) {
+                        const uint64_t o = order_of(order_key(v), i);
+                        if (o < floor || (top < 64 && (o >> top) != prefix)) return;
+                        const int b = (int)((o >> shift) & (uint64_t)(nb - 1));
+                        atomicAdd(&count[b], 1u);
+                        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(v)));
+                    });
+                    __syncthreads();
+                    const int b1 = nb - 1 - 2 * tid;                       // this thread's bins, the upper first
+                    uint64_t c[2], m[2], unused;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        c[j] = b1 - j >= 0 ? count[b1 - j] : 0;
+                        m[j] = b1 - j >= 0 ? mass[b1 - j] : 0;
+                    }
+                    uint64_t cb = above + block_scan<TOKEN_THREADS>(c[0] + c[1], part, unused) - c[0] - c[1];
+                    uint64_t mb = above_mass + block_scan<TOKEN_THREADS>(m[0] + m[1], part, unused) - m[0] - m[1];
+                    __syncthreads();
+                    if (tid == 0) shared_at = 0;
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const bool here = by_mass ? (double)mb < limit && !((double)(mb + m[j]) < limit)
+                                                  : cb < want && cb + c[j] >= want;
+                        if (here) {
+                            shared_at = b1 - j;
+                            shared_mass = mb;
+                            part[0] = cb;
+                        }
+                        cb += c[j];
+                        mb += m[j];
+                    }
+                    __syncthreads();
+                    prefix = (prefix << width) | (uint64_t)shared_at;
+                    above_mass = shared_mass;
+                    above = part[0];
+                    kept = above_mass + mass[shared_at];
+                    top = shift;
+                }
+                __syncthreads();
+                return prefix;
+            };
+            uint64_t total = 0;
+            least = 0;
+            if (x.top_k) least = search(false, 0, (uint32_t)x.top_k, 0.0, total);
+            if (x.by_mass) {
+                if (!x.top_k) {
+                    uint64_t sum = 0;
+                    for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
+                    block_scan<TOKEN_THREADS>(sum, part, total);
+                }
+                least = search(true, least, 0, mass_limit(x, total), total);
+            }
+            each([&](int i, float v) {
+                if (x.bin(v) < lo || order_of(order_key(v), i) < least) return;
+                const double w = x.weight(v);
+                if (w >= x.min_p || i == x.at) atomicAdd(&sums[i / TILE], (unsigned long long)x.fixed(w));
+            });
+        }
+    }
+    __syncthreads();
+    // the tile that the target falls into
+    uint64_t run_mass = 0, all = 0;
+    for (int t0 = 0; t0 < a.tiles; t0 += TOKEN_THREADS) {
+        uint64_t here;
+        const uint64_t v = t0 + tid < a.tiles ? (uint64_t)sums[t0 + tid] : 0;
+        block_scan<TOKEN_THREADS>(v, part, here);
+        all += here;
+    }
+    // (a random number of 1 or more: the last kept token)
+    const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
+    if (tid == 0) shared_at = -1;
+    for (int t0 = 0; t0 < a.tiles; t0 += TOKEN_THREADS) {
+        uint64_t here;
+        const uint64_t v = t0 + tid < a.tiles ? (uint64_t)sums[t0 + tid] : 0;
+        const uint64_t end = block_scan<TOKEN_THREADS>(v, part, here) + run_mass;
+        if (v && (double)(end - v) <= want && (double)end > want) {
+            shared_at = t0 + tid;
+            shared_mass = end - v;
+        }
+        run_mass += here;
+    }
+    __syncthreads();
+    const int tile = shared_at;
+    run_mass = shared_mass;
+    __syncthreads();
+    if (tile < 0) {                                      // (not reached: the first of the order has a weight)
+        if (tid == 0) a.out[r] = x.at;
+        return;
+    }
+    constexpr int E = TILE / TOKEN_THREADS;
+    uint64_t m[E], mine = 0, unused;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = tile * TILE + tid * E + e;
+        m[e] = 0;
+        if (i < a.vocab) {
+            const float v = to_f32(row[i]);
+            if (x.bin(v) < lo || order_of(order_key(v), i) >= least) {
+                const double w = x.weight(v);
+                if (w >= x.min_p || i == x.at) m[e] = x.fixed(w);
+            }
+        }
+        mine += m[e];
+    }
+    uint64_t before = run_mass + block_scan<TOKEN_THREADS>(mine, part, unused) - mine;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (m[e] && (double)before <= want && (double)(before + m[e]) > want) a.out[r] = tile * TILE + tid * E + e;
+        before += m[e];
+    }
 }
 
 }  // namespace kush
@@ -495,26 +750,73 @@ extern "C" int kush_step_maps(const int32_t* new_tokens, const int32_t* history,
     return kush_check_launch("kush_step_maps");
 }
 
+// Tiles of a row to a workgroup, for about three workgroups per CU
+static int64_t tiles_each(int64_t rows, int64_t tiles) { return std::min(tiles, (rows * tiles + 767) / 768); }
+
+constexpr int64_t SAMPLE_ROWS = 1024;            // rows of one launch; more go in turn, over the same scratch
+
+// Scratch of a launch, by 16-byte aligned pieces
+struct SampleScratch {
+    int64_t parts, mass, sums, count, length, list, bytes;
+    SampleScratch(int64_t rows, int64_t vocab) {
+        const int64_t tiles = (vocab + TILE - 1) / TILE;
+        int64_t at = 0;
+        const auto piece = [&](int64_t n) {
+            const int64_t p = at;
+            at = (at + n + 15) & ~int64_t(15);
+            return p;
+        };
+        parts = piece(rows * tiles * (int64_t)sizeof(SamplePart));
+        mass = piece(rows * BINS * 8);
+        sums = piece(rows * tiles * 8);
+        count = piece(rows * BINS * 4);
+        length = piece(rows * 4);
+        list = piece(rows * LIST * 8);
+        bytes = at;
+    }
+};
+
+extern "C" int64_t kush_sample_scratch(int64_t rows, int64_t vocab) {
+    if (rows < 0 || vocab < 1 || vocab > (1 << 24)) return 0;
+    return SampleScratch(std::min(rows, SAMPLE_ROWS), vocab).bytes;
+}
+
 extern "C" int kush_sample(int dtype, const void* logits, int64_t row_stride, int64_t rows, int64_t vocab,
                            const float* uniforms, double temperature, const float* temperatures, int32_t top_k,
                            const int32_t* top_ks, double top_p, const float* top_ps, double min_p, const float* min_ps,
-                           int64_t* out, void* stream) {
+                           int64_t* out, void* scratch, int64_t scratch_bytes, void* stream) {
     if (rows < 0 || rows > 0x7fffffff || vocab < 1 || vocab > (1 << 24) || row_stride < 0)
         return kush_fail(-2, "kush_sample: bad rows %lld / vocab %lld (1 .. 2^24) / row_stride %lld", (long long)rows,
                          (long long)vocab, (long long)row_stride);
     if (dtype < 0 || dtype > 2) return kush_fail(-1, "kush_sample: unsupported dtype code %d (0 fp32, 1 fp16, 2 bf16)", dtype);
     if (rows == 0) return 0;
+    const SampleScratch at(std::min(rows, SAMPLE_ROWS), vocab);
+    if (scratch == nullptr || ((uintptr_t)scratch & 15) || scratch_bytes < at.bytes)
+        return kush_fail(-2, "kush_sample: needs %lld bytes of 16-byte aligned scratch (kush_sample_scratch)", (long long)at.bytes);
     int log = 0;
     while ((1ll << log) < vocab) ++log;
-    const SampleArgs a{logits,      row_stride, (int)vocab,   61 - log, uniforms, temperature, top_p, min_p, top_k,
-                       temperatures, top_ps,     min_ps,       top_ks,   out};
-    const dim3 grid((unsigned)rows), block(SAMPLE_THREADS);
+    uint8_t* const base = (uint8_t*)scratch;
+    SampleArgs a{logits,       row_stride, (int)vocab, std::min(50, 61 - log), (int)((vocab + TILE - 1) / TILE),
+                 0,            uniforms,   temperature, top_p,                 min_p,
+                 top_k,        temperatures, top_ps,   min_ps,                 top_ks,
+                 out,          (SamplePart*)(base + at.parts),                 (uint64_t*)(base + at.mass),
+                 (uint64_t*)(base + at.sums), (uint32_t*)(base + at.count),    (uint32_t*)(base + at.length),
+                 (uint2*)(base + at.list),    0};
+    const bool cuts = top_ks || top_ps || top_k > 0 || top_p < 1.0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == 0)
-        sample_kernel<float><<<grid, block, 0, st>>>(a);
-    else if (dtype == 1)
-        sample_kernel<_Float16><<<grid, block, 0, st>>>(a);
-    else
-        sample_kernel<bf16_t><<<grid, block, 0, st>>>(a);
-    return kush_check_launch("kush_sample");
+    const auto go = [&](auto in) {
+        using T = decltype(in);
+        for (; a.row0 < rows; a.row0 += SAMPLE_ROWS) {
+            const int64_t n = std::min(SAMPLE_ROWS, rows - a.row0);
+            a.per = (int)tiles_each(n, a.tiles);
+            const int pieces = (a.tiles + a.per - 1) / a.per;
+            const dim3 grid((unsigned)pieces, (unsigned)n);
+            sample_max<T><<<grid, dim3(PIECE_THREADS), 0, st>>>(a);
+            if (cuts) sample_bins<T><<<grid, dim3(PIECE_THREADS), 0, st>>>(a);
+            sample_pick<T><<<grid, dim3(PIECE_THREADS), 0, st>>>(a);
+            sample_token<T><<<dim3((unsigned)n), dim3(TOKEN_THREADS), 0, st>>>(a, pieces);
+        }
+        return kush_check_launch("kush_sample");
+    };
+    return dtype == 0 ? go(float{}) : (dtype == 1 ? go(_Float16{}) : go(bf16_t{}));
 }
