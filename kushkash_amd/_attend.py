@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 
 import torch
 
@@ -131,6 +132,32 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
     return 4, chunk
 
 
+@lru_cache(512)
+def _window_plan(spans: tuple, group: int, hkv: int, D: int, total: int, scratch: int, window: int, sinks: int) -> tuple[int, int, int]:
+    """plan() under a window, and the rows that the partials of split keys take (a step's layers ask for the same)."""
+    waves, chunk = plan(spans, group, hkv, D, total, True, scratch, window, sinks)
+    if not chunk:
+        return waves, 0, 0
+    tiles = min(-(-max(n for _, n, _ in spans) // KEYS), window_tiles(window, sinks, 32 * waves, group))
+    return waves, chunk, -(-tiles // chunk) * total * hkv * group
+
+
+def _native(q, k, v, scale, cu, spans, out, scratch, window, sinks):
+    """A windowed call in native code (csrc/kush_stepcall.cpp), or None: not taken, nothing was launched."""
+    m = _lib.native()
+    n_k = k.shape[1] if cu is None else cu[3]
+    if m is None or window >= n_k:
+        return None
+    if cu is None:
+        n_q, total, cu = q.shape[1], q.shape[0] * q.shape[1], (None, None)
+        shape = ((n_q, n_k, q.shape[0]),)
+    else:
+        n_q, total, shape = cu[2], q.shape[0], tuple((t, n, 1) for t, n in spans)
+    waves, chunk, rows = _window_plan(shape, q.shape[-2] // k.shape[-2], k.shape[-2], q.shape[-1], total, scratch, window, sinks)
+    return m.attend(q, k, v, out, cu[0], cu[1], n_q, n_k, scale, window, sinks, waves, chunk, rows,
+                    torch._C._cuda_getCurrentRawStream(q.get_device()))
+
+
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float, lse: bool = False,
            cu: tuple | None = None, spans=None, out: torch.Tensor | None = None, scratch: int = PARTIAL_BYTES,
            window: int = 0, sinks: int = 0):
@@ -141,6 +168,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scal
     `window` and the first `sinks` (0: all of them)."""
     D, Hq, Hk = q.shape[-1], q.shape[-2], k.shape[-2]
     group = Hq // Hk
+    if window and not lse and (o := _native(q, k, v, scale, cu, spans, out, scratch, window, sinks)) is not None:
+        return o
     if cu is None:
         seqs, n_q, n_k, total = q.shape[0], q.shape[1], k.shape[1], q.shape[0] * q.shape[1]
         cq = ck = None

@@ -117,6 +117,27 @@ def fastcall():
     return _fastcall
 
 
+@lru_cache(None)
+def stepcall():
+    """The native host calls around a windowed step (csrc/kush_stepcall.cpp), bound to the library, or None where they are not
+    built: every call then checks its arguments in Python."""
+    try:
+        from . import _stepcall
+    except ImportError:
+        return None
+    if getattr(_stepcall, "ABI", None) != ABI_VERSION:
+        raise RuntimeError(f"kushkash_amd: _stepcall.so is for ABI {getattr(_stepcall, 'ABI', None)}, expected {ABI_VERSION}; "
+                           "rebuild it")
+    _stepcall.bind(check, *(address(n) for n in ("kush_window_decode", "kush_window_attend", "kush_block_table",
+                                                 "kush_step_maps", "kush_sample", "kush_sample_scratch")))
+    return _stepcall
+
+
+def native():
+    """stepcall(), but not where the library calls are recorded or replaced (call)."""
+    return stepcall() if call is PLAIN_CALL else None
+
+
 def call(name: str, *args) -> None:
     """Run one entry point; -1 (unsupported shape) -> ValueError like the reference's CPU path
     (kushkash/_cpu.py:38-40), any other failure -> RuntimeError with the library's message."""

@@ -180,6 +180,7 @@ class Ops:
         # counters of the fused split-K merge: zero at rest (the last workgroup of each (sequence, kv
         # head) resets its own), so one buffer serves every call of this Ops on one stream at a time
         self._sync = torch.zeros(SYNC_SLOTS, dtype=torch.int32, device=self.device)
+        self._sync_address = self._sync.data_ptr()
         self._fast = _lib.fastcall()
         if self._fast is not None:
             self._config = self._fast.make_config(
@@ -212,6 +213,18 @@ class Ops:
         if rc != self._fast.NOT_TAKEN:
             self._lib.check("kush_decode_ex" if k is None else "kush_append_decode", rc)
         return False
+
+    def _native_window(self, k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order,
+                       rot, window, sinks) -> bool:
+        """_native_decode under a window."""
+        m = self._lib.native() if self.gpu and not self.validate else None
+        if m is None:
+            return False
+        if waves is None:
+            waves = self.waves(q.shape[0], tail_k.shape[1], n_splits)
+        return m.decode(self.D, self.bits, self.G, self._dt, self.device.index, self._sync_address, SYNC_SLOTS, k, v, q, out,
+                        cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot, window, sinks,
+                        torch._C._cuda_getCurrentRawStream(self.device.index)) is not None
 
     def _on_device(self, **ts: torch.Tensor) -> None:
         for name, t in ts.items():
@@ -481,8 +494,10 @@ class Ops:
         (splits(window=, sinks=))."""
         window, sinks = check_limit(window, sinks)
         if window:
-            self._decode(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot,
-                         None, None, window, sinks)
+            if not self._native_window(None, None, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits,
+                                       work, waves, order, rot, window, sinks):
+                self._decode(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, waves, order, rot,
+                             None, None, window, sinks)
             return
         if self._native() and self._native_decode(None, None, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale,
                                                   n_splits, work, waves, order, rot):
@@ -502,6 +517,9 @@ class Ops:
         decode. No reference counterpart."""
         window, sinks = check_limit(window, sinks)
         limit = {"window": window, "sinks": sinks} if window else {}
+        if window and self._native_window(k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work,
+                                          waves, order, rot, window, sinks):
+            return
         if not window and self._native() and self._native_decode(k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale,
                                                   n_splits, work, waves, order, rot):
             return

@@ -20,6 +20,13 @@ def _call(name: str, device: torch.device, *args) -> None:
         _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
+def _native(name: str, first: torch.Tensor, *args):
+    """The call's result in native code, or None: not taken, nothing was launched."""
+    from . import _lib
+    m = _lib.native()
+    return None if m is None else getattr(m, name)(first, *args, torch._C._cuda_getCurrentRawStream(first.get_device()))
+
+
 def _index(name: str, t: torch.Tensor, n: int, device: torch.device, dtypes=(torch.int32,)) -> None:
     if t.dtype not in dtypes or not t.is_contiguous() or t.dim() != 1 or t.numel() != n or t.device != device:
         raise ValueError(f"{name} must be contiguous {' or '.join(str(d).split('.')[1] for d in dtypes)} [{n}] on {device}, "
@@ -42,6 +49,8 @@ def block_table(req_to_token: torch.Tensor, req: torch.Tensor, seq_lens: torch.T
     [map rows, context], a token's slot being its block * 32 + its row in the page) read at rows req [R] for the pages
     that seq_lens [R] (both int32 or int64) reach; 0 behind them, and where req or a length is outside the map. slots is
     req. out: the three arrays to fill (a captured step's static buffers; the table's rows may be strided)."""
+    if req_to_token.is_cuda and (got := _native("block_table", req_to_token, req, seq_lens, pages, out)) is not None:
+        return got
     dev, R = req_to_token.device, req.numel()
     _map("req_to_token", req_to_token, None, dev)
     _index("req", req, R, dev, _INDEX)
@@ -85,6 +94,10 @@ class MapSizes:
     tails: int
     window: int = 0
     sinks: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "numbers", (self.requests, self.tokens, self.keys, self.jobs, self.pages, self.tails,
+                                             self.window, self.sinks))
 
 
 @dataclass
@@ -132,6 +145,8 @@ def step_maps(new_tokens: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     tail in slot slots[r] (int32 [R]) and its pages in block_table[r] (int32 [R, pages]): what Ops.write, Ops.unpack and the
     ragged attention of the step take. sizes: map_sizes of the same lengths, which the host knows before the step. Lengths
     on the device that need more than the sizes hold are cut off at them."""
+    if new_tokens.is_cuda and (got := _native("step_maps", new_tokens, history, slots, block_table, sizes.numbers)) is not None:
+        return StepMaps(*got)
     dev, R = new_tokens.device, sizes.requests
     for name, t in (("new_tokens", new_tokens), ("history", history), ("slots", slots)):
         _index(name, t, R, dev)
@@ -216,6 +231,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     exceeds the random number times the sum of all: the same for the same inputs, on every call. temperature 0 takes
     the first of the order. A row with a NaN, or without a logit above -inf, gives -1. Each setting is a number, or a tensor
     with one per row (fp32; top_k int32). On the GPU."""
+    if logits.is_cuda and (got := _native("sample", logits, uniforms, temperature, top_k, top_p, min_p, out)) is not None:
+        return got
     if logits.dim() != 2 or logits.dtype not in _CODE or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits must be fp32, fp16 or bf16 [rows, vocabulary] with unit column stride, got {logits.dtype} "
                          f"{tuple(logits.shape)}")

@@ -36,6 +36,9 @@ CPU_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", "-fopenmp", "-ffp-contract
 # The native host side of the per-step calls (csrc/kush_fastcall.cpp, a Python extension over torch's headers)
 FAST_LIB = PKG / "_fastcall.so"
 FAST_SOURCE = "kush_fastcall.cpp"
+# and of the calls around a windowed step
+STEP_LIB = PKG / "_stepcall.so"
+STEP_SOURCE = "kush_stepcall.cpp"
 FAST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 SOURCES = ("kush_capi.hip", "kush_write.hip", "kush_decode.hip", "kush_rotate.hip",
            "kush_unpack.hip", "kush_attend.hip", "kush_window_attend.hip", "kush_step.hip", "kush_decode_inst.hip",
@@ -130,7 +133,7 @@ def source_digest(unit: str | None = None) -> str:
         files = sorted(seen)
     for f in files:
         h.update(f.name.encode() + b"\0" + _code(f.read_text()).encode() + b"\0")
-    h.update(repr({CPU_SOURCE: CPU_FLAGS, FAST_SOURCE: FAST_FLAGS}.get(unit, (FLAGS, units()))).encode())
+    h.update(repr({CPU_SOURCE: CPU_FLAGS, FAST_SOURCE: FAST_FLAGS, STEP_SOURCE: FAST_FLAGS}.get(unit, (FLAGS, units()))).encode())
     return h.hexdigest()[:16]
 
 
@@ -170,8 +173,8 @@ def cxx() -> str:
     raise RuntimeError("g++ not found (the CPU path's library is built with it)")
 
 
-def fastcall_command(out: Path) -> list[str]:
-    """The compiler call that builds FAST_SOURCE against the torch it will run with."""
+def fastcall_command(out: Path, source: str = FAST_SOURCE) -> list[str]:
+    """The compiler call that builds FAST_SOURCE (or STEP_SOURCE) against the torch it will run with."""
     import sysconfig
 
     import torch
@@ -181,13 +184,13 @@ def fastcall_command(out: Path) -> list[str]:
     return [cxx(), *FAST_FLAGS, f"-DKUSH_FASTCALL_ABI={ABI_VERSION}", f"-I{ROOT / 'include'}", f"-I{base / 'include'}",
             f"-I{base / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", str(out),
-            str(PKG / "csrc" / FAST_SOURCE), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            str(PKG / "csrc" / source), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     """Compile every HIP source for gfx950 into LIB, TIMELINE_LIB from the same objects with the
     timeline unit instrumented, the measurement library FLOOR_LIB, the CPU path's host library
-    CPU_LIB and the native host calls FAST_LIB (always recompiles; objects in parallel, then the links); returns LIB."""
+    CPU_LIB and the native host calls FAST_LIB and STEP_LIB (always recompiles; objects in parallel, then the links); returns LIB."""
     todo = units() + [(FLOOR_SOURCE, {}), (TIMELINE_UNIT[0], dict(TIMELINE_UNIT[1], KUSH_TIMELINE=1))]
     jobs = jobs or max(1, min(len(todo), int(os.environ.get("MAX_JOBS", 0)) or os.cpu_count() or 1))
     compile_flags = [f for f in FLAGS if f != "-shared"]
@@ -202,10 +205,13 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
         cmds.append([cxx(), *CPU_FLAGS, f"-I{ROOT / 'include'}", "-o", str(cpu_tmp), str(PKG / "csrc" / CPU_SOURCE)])
         fast_tmp = FAST_LIB.with_suffix(".so.tmp")
         cmds.append(fastcall_command(fast_tmp))
+        step_tmp = STEP_LIB.with_suffix(".so.tmp")
+        cmds.append(fastcall_command(step_tmp, STEP_SOURCE))
         with ThreadPoolExecutor(jobs) as ex:
             list(ex.map(lambda c: _run(c, verbose), cmds))
         os.replace(cpu_tmp, CPU_LIB)
         os.replace(fast_tmp, FAST_LIB)
+        os.replace(step_tmp, STEP_LIB)
         product = objs[:len(units())]
         swap = units().index(TIMELINE_UNIT)
         timeline = product[:swap] + objs[-1:] + product[swap + 1:]
@@ -215,7 +221,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
             os.replace(tmp, dst)
     import json
     DIGEST.write_text(json.dumps({"all": source_digest(),
-                                  **{u: source_digest(u) for u in SOURCES + (FLOOR_SOURCE, CPU_SOURCE, FAST_SOURCE)}},
+                                  **{u: source_digest(u) for u in SOURCES + (FLOOR_SOURCE, CPU_SOURCE, FAST_SOURCE, STEP_SOURCE)}},
                                  indent=1) + "\n")
     return LIB
 
