@@ -16,14 +16,15 @@ extern "C" {
 /* kush_decode_ex under a window: each sequence's query is its newest token (position seq_lens[s] - 1). With k and v (row
  * s the token at that position, rows 16-byte aligned, group <= 16) the token is appended first, as kush_append_decode
  * does; both null: the cache holds it already. Only the pages that are seen are read, and only their block_table
- * entries: a page between the sinks and the window may hold anything, or another sequence's tokens. n_splits counts over
- * the pages that are seen. waves: 0, 2 or 4 (8 runs 4). */
+ * entries (with bt_cols > 0 the other entries of a row are loaded too, and not used): a page between the sinks and the
+ * window may hold anything, or another sequence's tokens. n_splits counts over the pages that are seen. waves: 0, 2 or 4 (8 runs 4). */
 int kush_window_decode(int head_dim, int bits, int group, int dtype, const void* q, void* out, void* cache,
                        int64_t block_stride, int64_t head_stride, void* tail_k, const int32_t* tail_idx,
                        const int32_t* block_table, const int32_t* seq_lens, int64_t bt_row_stride, int32_t hkv,
                        float scale, int32_t n_splits, float* part_ml, float* part_o, int32_t n_seqs, void* stream,
-                       const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride, int32_t* split_sync,
-                       int32_t waves, const int32_t* seq_order, int32_t rot, int32_t window, int32_t sinks);
+                       const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride, int32_t bt_cols,
+                       int32_t* split_sync, int32_t waves, const int32_t* seq_order, int32_t rot, int32_t window,
+                       int32_t sinks);
 
 /* kush_attend (kushkash_amd_attend.h) of queries that are the last of their keys, under a window: query row t of a
  * sequence with T rows and N >= T keys is position N - T + t. Keys left out of the rows between the sinks and the first

@@ -66,8 +66,8 @@ ATTEND_SIGNATURES = {
 }
 # include/kushkash_amd_window.h
 WINDOW_SIGNATURES = {
-    # the decode list, then k, v, k_row_stride, v_row_stride, split_sync, waves, seq_order, rot, window, sinks
-    "kush_window_decode": _DECODE + [_P, _P, _I64, _I64, _P, _I32, _P, _I32, _I32, _I32],
+    # the decode list, then k, v, k_row_stride, v_row_stride, then the decode extensions, window, sinks
+    "kush_window_decode": _DECODE + [_P, _P, _I64, _I64] + _DECODE_EXT + [_I32, _I32],
     # kush_attend's list without causal, then window, sinks
     "kush_window_attend": [_I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F, _I32, _I32,
                            _I32, _P, _P, _P, _I32, _I32],

@@ -592,7 +592,7 @@ class Ops:
         if window:
             rows = (None, None, 0, 0) if app_k is None else (app_k.data_ptr(), app_v.data_ptr(), app_k.stride(0),
                                                              app_v.stride(0))
-            self._lib.call("kush_window_decode", *ref, *rows, *ext[1:], window, sinks)
+            self._lib.call("kush_window_decode", *ref, *rows, *ext, window, sinks)
         elif app_k is None:
             self._lib.call("kush_decode_ex", *ref, *ext)
         else:

@@ -8,6 +8,7 @@ from dataclasses import dataclass
 
 import torch
 
+from . import _lib
 from ._window import PAGE, check_limit, pages_left_out
 
 _INDEX = (torch.int32, torch.int64)
@@ -15,14 +16,12 @@ MOST_REQUESTS = 1 << 16
 
 
 def _call(name: str, device: torch.device, *args) -> None:
-    from . import _lib
     with torch.cuda.device(device):
         _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
 def _native(name: str, first: torch.Tensor, *args):
     """The call's result in native code, or None: not taken, nothing was launched."""
-    from . import _lib
     m = _lib.native()
     return None if m is None else getattr(m, name)(first, *args, torch._C._cuda_getCurrentRawStream(first.get_device()))
 
@@ -254,7 +253,6 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         out = torch.empty(B, dtype=torch.int64, device=dev)
     _index("out", out, B, dev, (torch.int64,))
     if B:
-        from . import _lib
         scratch = torch.empty(_lib.lib().kush_sample_scratch(B, V), dtype=torch.uint8, device=dev)
         _call("kush_sample", dev, _CODE[logits.dtype], logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V,
               uniforms.data_ptr(), *settings, out.data_ptr(), scratch.data_ptr(), scratch.numel())

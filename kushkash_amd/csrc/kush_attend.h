@@ -227,7 +227,7 @@ __global__ __launch_bounds__(NW * WAVE) void attend_kernel(const Args a) {
     const int whi = first >= rows ? -1 : (a.causal ? off + min(first + 31, rows - 1) / G : s.N - 1);
 
     s8 qf[KS];                                                           // B operand: row r32, dims 16 ks + 8 hh ..
-    {
+    if constexpr (!windowed<Args>) {
         const uint16_t* qp = (const uint16_t*)a.q + s.q + t * a.q_row + (int64_t)(h * G + g) * a.q_head + 8 * hh;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const s8*>(qp + 16 * ks);
@@ -283,10 +283,19 @@ __global__ __launch_bounds__(NW * WAVE) void attend_kernel(const Args a) {
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
     float mr = -__builtin_inff(), l = 0.0f;                              // running max (log2 units), this half's sum
 
+    if constexpr (windowed<Args>) {                                      // few tiles: the first ones go out ahead of q
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) issue(j0 + i, i);
+        const uint16_t* qp = (const uint16_t*)a.q + s.q + t * a.q_row + (int64_t)(h * G + g) * a.q_head + 8 * hh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const s8*>(qp + 16 * ks);
+    }
     __builtin_amdgcn_s_waitcnt(0x0F70);                                 // q is in: only DMAs count in vmcnt below
     asm volatile("" ::: "memory");
+    if constexpr (!windowed<Args>) {
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) issue(j0 + i, i);
+        for (int i = 0; i < ST - 1; ++i) issue(j0 + i, i);
+    }
     int st = 0;
     for (int i = j0; i < j1; ++i) {
         // tile i is in and, behind the barrier, in for every wave, and every wave has read tile i - 1, whose

@@ -1072,6 +1072,7 @@ struct View {
     static constexpr int gap = 0;
     __device__ __forceinline__ View(int) {}
     __device__ __forceinline__ int page(int p) const { return p; }
+    __device__ __forceinline__ int index(int p) const { return p; }
     __device__ __forceinline__ bool hidden(int) const { return false; }
 };
 template <>
@@ -1086,6 +1087,8 @@ struct View<true> {
         count = (uint32_t)max(0, begin - gap * PAGE - sinks);
     }
     __device__ __forceinline__ int page(int p) const { return p < first ? p : p + gap; }
+    // the list index of logical page p, -1 for one that is left out
+    __device__ __forceinline__ int index(int p) const { return p < first ? p : (p < first + gap ? -1 : p - gap); }
     __device__ __forceinline__ bool hidden(int t) const { return (uint32_t)(t - lo) < count; }
     // whether any of n tokens from t on are hidden
     __device__ __forceinline__ bool hides(int t, int n) const { return count != 0 && lo < t + n && t < lo + (int)count; }
@@ -1229,10 +1232,12 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
     if (app_k != nullptr && zg == NSG - 1 && w == aw)
         token.load(app_k + (int64_t)s * app_ks + (int64_t)h * D, app_v + (int64_t)s * app_vs + (int64_t)h * D, lane);
     constexpr int PRE = WIN / (NW * WAVE);                               // prefetched ids per thread
-    const int npre = !ws && !WN && z == 0 ? min(WIN, bt_cols) : 0;      // (WN: the pages depend on the length)
+    // (WN: which pages a split takes depends on the length: the whole row of a table of up to PREN columns per thread)
+    constexpr int PREN = WN && PRE > 4 ? 4 : PRE;
+    const int npre = WN ? (bt_cols <= PREN * NW * WAVE ? bt_cols : 0) : !ws && z == 0 ? min(WIN, bt_cols) : 0;
     int pre[PRE];
 #pragma unroll
-    for (int k = 0; k < PRE; ++k) {
+    for (int k = 0; k < PREN; ++k) {
         const int i = (int)threadIdx.x + k * NW * WAVE;
         pre[k] = i < npre ? bt[i] : 0;
     }
@@ -1353,7 +1358,13 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
         const int PS = ws ? 1 : NW;                                      // the wave's pair stride
         int wb = p0, wn = min(TW, p1 - p0), pairs = (wn + 1) / 2;
         const auto load_window = [&]() {
-            if (wb == 0 && wn <= npre) {                                 // split 0's first window, prefetched
+            if (WN && npre > 0) {                                        // the row, prefetched: this window's part of the list
+#pragma unroll
+                for (int k = 0; k < PREN; ++k) {
+                    const int i = (int)threadIdx.x + k * NW * WAVE, at = view.index(i) - wb;
+                    if (at >= 0 && at < wn) tbl[at] = pre[k];
+                }
+            } else if (wb == 0 && wn <= npre) {                          // split 0's first window, prefetched
 #pragma unroll
                 for (int k = 0; k < PRE; ++k) {
                     const int i = (int)threadIdx.x + k * NW * WAVE;
@@ -1463,7 +1474,9 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
             float sv[8], kx;                                                                       \
             pair_scores2<D, BITS, QLO>(SA, qa, qla, qh, ql, sv, kx, rs, lane);                     \
             if (2 * (P) + 1 >= wn && r16 >= 8) kx = -__builtin_inff();   /* page B masked */        \
-            if constexpr (WN) view.mask(sv, (wb + 2 * (P) + (r16 >> 3)) * PAGE, q);                \
+            if constexpr (WN) {                                                                    \
+                if (view.hides((wb + 2 * (P)) * PAGE, 2 * PAGE)) view.mask(sv, (wb + 2 * (P) + (r16 >> 3)) * PAGE, q); \
+            }                                                                                      \
             id2 = *reinterpret_cast<const int2*>(tb + min(2 * nx, TW - 2));                        \
             consume2<D, BITS, vpre<D, BITS, DEP, WS>()>(SA, R::SLOT, o, vacc, sv, sa, kx, m_run, l_run, vb_run, lane);       \
         } else {                                                                                   \
@@ -1477,8 +1490,10 @@ __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(2, D 
             const float pbm = 2 * (P) + 1 >= wn ? -__builtin_inff() : 0.0f;                        \
             _Pragma("unroll") for (int jj = 0; jj < 8; ++jj) sv[1][jj] += pbm;                     \
             if constexpr (WN) {                                                                    \
-                view.mask(sv[0], (wb + 2 * (P)) * PAGE, q);                                        \
-                view.mask(sv[1], (wb + 2 * (P) + 1) * PAGE, q);                                    \
+                if (view.hides((wb + 2 * (P)) * PAGE, 2 * PAGE)) {                                 \
+                    view.mask(sv[0], (wb + 2 * (P)) * PAGE, q);                                    \
+                    view.mask(sv[1], (wb + 2 * (P) + 1) * PAGE, q);                                \
+                }                                                                                  \
             }                                                                                      \
             id2 = *reinterpret_cast<const int2*>(tb + min(2 * nx, TW - 2));                        \
             consume_pages<D, BITS, 2, vpre<D, BITS, DEP, WS>()>(sp, o, vacc, sv, sa, kx, m_run, l_run, vb_run, lane);        \

@@ -163,8 +163,8 @@ extern "C" int kush_window_decode(int head_dim, int bits, int group, int dtype, 
                                   const int32_t* block_table, const int32_t* seq_lens, int64_t bt_stride, int32_t hkv,
                                   float scale, int32_t n_splits, float* part_ml, float* part_o, int32_t n_seqs,
                                   void* stream, const void* k, const void* v, int64_t k_row_stride,
-                                  int64_t v_row_stride, int32_t* split_sync, int32_t waves, const int32_t* seq_order,
-                                  int32_t rot, int32_t window, int32_t sinks) {
+                                  int64_t v_row_stride, int32_t bt_cols, int32_t* split_sync, int32_t waves,
+                                  const int32_t* seq_order, int32_t rot, int32_t window, int32_t sinks) {
     if (window <= 0 || sinks < 0) return kush_fail(-2, "kush_window_decode: bad window %d / sinks %d", window, sinks);
     if ((k == nullptr) != (v == nullptr)) return kush_fail(-2, "kush_window_decode: k and v go together");
     if (k != nullptr && group > 16)
@@ -174,7 +174,7 @@ extern "C" int kush_window_decode(int head_dim, int bits, int group, int dtype, 
         (((uintptr_t)k | (uintptr_t)v | (uint64_t)(k_row_stride * e) | (uint64_t)(v_row_stride * e)) & 15))
         return kush_fail(-2, "kush_window_decode: k / v rows must be 16-byte aligned (append first: k and v null)");
     return decode_impl("kush_window_decode", head_dim, bits, group, dtype, q, out, cache, block_stride, head_stride, tail_k,
-                       tail_idx, block_table, seq_lens, bt_stride, 0, hkv, scale, n_splits, part_ml, part_o, split_sync,
+                       tail_idx, block_table, seq_lens, bt_stride, bt_cols, hkv, scale, n_splits, part_ml, part_o, split_sync,
                        waves, seq_order, n_seqs, rot, Append{k, v, k_row_stride, v_row_stride}, stream,
                        Window{window, sinks});
 }

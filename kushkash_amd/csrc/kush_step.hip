@@ -164,6 +164,9 @@ struct SamplePart {
 };
 
 constexpr int BINS = 1024, TILE = 4096, LIST = 8192, PIECE_THREADS = 256;
+// top_k up to here: the list takes every token down to the class of top-k's cut, so that the bins need no masses (150,000
+// tokens x 64 rows, top_k 240 - 400, top_p: 28.2 us for the bins with masses)
+constexpr int SMALL_K = 2048;
 constexpr float SPAN = 64.0f;        // logits (in units of max(1, T)) that the bins cover at most
 
 // logits in an order of their own: larger logit, larger key; -0 and 0 alike
@@ -190,7 +193,7 @@ struct SampleRow {
     double c, top_p, min_p;          // c = log2 e / T
     float most, scale;               // scale: bins per logit
     int top_k, at;                   // top_k 0: off; at: the first of the order
-    bool none, greedy, by_mass;
+    bool none, greedy, by_mass, bin_mass;        // bin_mass: top-p is cut by the bins' masses
     int bits;
     __device__ __forceinline__ double weight(float x) const { return exp2_64(x == most ? 0.0 : ((double)x - (double)most) * c); }
     // w >= 0 in multiples of 2^-bits, at least one where w is above 0
@@ -245,12 +248,28 @@ __device__ __forceinline__ SamplePart merge_parts(SamplePart a, const SamplePart
     a.nan |= b.nan;
     return a;
 }
+// op over the wave's lanes, in all of them, on the VALU
+template <typename Op>
+__device__ __forceinline__ float wave_all(float x, Op&& op) {
+    x = op(x, lane_xor<1>(x));
+    x = op(x, lane_xor<2>(x));
+    x = op(x, lane_xor<4>(x));
+    x = op(x, lane_xor<8>(x));
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ SamplePart wave_part(SamplePart p) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1)
-        p = merge_parts(p, SamplePart{__shfl_xor(p.most, m, WAVE), __shfl_xor(p.least, m, WAVE), __shfl_xor(p.at, m, WAVE),
-                                      __shfl_xor(p.nan, m, WAVE)});
-    return p;
+    const auto larger = [](float u, float v) { return __builtin_fmaxf(u, v); };
+    const auto smaller = [](float u, float v) { return __builtin_fminf(u, v); };
+    SamplePart r;
+    r.most = wave_all(p.most, larger);
+    r.least = wave_all(p.least, smaller);
+    const auto first = [](float u, float v) { return __int_as_float(min(__float_as_int(u), __float_as_int(v))); };
+    r.at = __float_as_int(wave_all(__int_as_float(p.most == r.most ? p.at : 0x7fffffff), first));
+    r.nan = __any(p.nan);
+    return r;
 }
 constexpr SamplePart NO_PART{-__builtin_inff(), __builtin_inff(), 0x7fffffff, 0};
 
@@ -301,6 +320,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, 
     const int k = a.top_ks ? a.top_ks[r] : a.top_k;
     x.top_k = k > 0 && k < a.vocab ? k : 0;
     x.by_mass = x.top_p < 1.0;
+    x.bin_mass = x.by_mass && !(x.top_k && x.top_k <= SMALL_K);
     x.none = p.nan || p.most == -__builtin_inff();
     x.greedy = !(temp > 0.0);
     x.most = p.most;
@@ -336,14 +356,14 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_bins(const SampleArgs a)
                 if (i + e >= a.vocab) continue;
                 const int b = x.bin(c.x[e]);
                 atomicAdd(&count[b], 1u);
-                if (x.by_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(c.x[e])));
+                if (x.bin_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(c.x[e])));
             }
         });
     __syncthreads();
     for (int i = tid; i < BINS; i += PIECE_THREADS)
         if (count[i]) {
             atomicAdd(&a.count[s * BINS + i], count[i]);
-            if (x.by_mass) atomicAdd((unsigned long long*)&a.mass[s * BINS + i], (unsigned long long)mass[i]);
+            if (x.bin_mass) atomicAdd((unsigned long long*)&a.mass[s * BINS + i], (unsigned long long)mass[i]);
         }
 }
 
@@ -386,24 +406,26 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
     __shared__ SampleCuts cuts;
     constexpr int N = BINS / THREADS;
     const int tid = threadIdx.x;
-    uint32_t c[N];
-    uint64_t m[N], cs = 0, ms = 0, c_all, m_all;
+    uint32_t c[N], cs = 0, c_all;
+    uint64_t m[N], ms = 0, m_all = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         c[i] = a.count[s * BINS + tid * N + i];
-        m[i] = x.by_mass ? a.mass[s * BINS + tid * N + i] : 0;
+        m[i] = x.bin_mass ? a.mass[s * BINS + tid * N + i] : 0;
         cs += c[i];
         ms += m[i];
     }
     if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0};
-    const uint64_t c1 = block_scan<THREADS>(cs, part, c_all), m1 = block_scan<THREADS>(ms, part, m_all);
+    const uint32_t c1 = block_scan<THREADS>(cs, reinterpret_cast<uint32_t*>(part), c_all);
+    const uint64_t m1 = x.bin_mass ? block_scan<THREADS>(ms, part, m_all) : 0;
     if (x.top_k) {
-        uint64_t cb = c1 - cs, mb = m1 - ms;
+        uint32_t cb = c1 - cs;
+        uint64_t mb = m1 - ms;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (cb < (uint64_t)x.top_k && cb + c[i] >= (uint64_t)x.top_k) {
+            if (cb < (uint32_t)x.top_k && cb + c[i] >= (uint32_t)x.top_k) {
                 cuts.k = tid * N + i;
-                cuts.above_k = (uint32_t)cb;
+                cuts.above_k = cb;
                 cuts.before_k = mb;
             }
             cb += c[i];
@@ -413,8 +435,11 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
     __syncthreads();
     const SampleCuts now = cuts;
     __syncthreads();
-    if (!x.by_mass) {
-        if (tid == 0) cuts.lo = cuts.hi = now.k;
+    if (!x.bin_mass) {
+        if (tid == 0) {
+            cuts.lo = x.by_mass ? 0 : now.k;                    // top-p as well: the list takes all that top-k keeps
+            cuts.hi = now.k;
+        }
     } else {
         // the kept mass lies between what is below k and what k adds: so does top-p's cut
         uint64_t mb = m1 - ms;
@@ -436,9 +461,15 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
     return cuts;
 }
 
+// Tokens of the list that a workgroup gathers in LDS before it takes places in the row's: a tile may hold TILE of them, and
+// a place of its own for each wave's tokens costs a trip to memory and back (102 us at 64 rows of 600 tokens each; 19 so)
+constexpr int GATHER = TILE + 1024;
+
 template <typename T>
 __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a) {
+    __shared__ uint2 gather[GATHER];
     __shared__ unsigned long long sum;
+    __shared__ uint32_t held, place;
     const int64_t s = blockIdx.y, r = a.row0 + s;
     const int piece = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE;
     const SampleRow x = sample_row(a, s, gridDim.x);
@@ -446,9 +477,14 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
     SampleCuts cut{BINS, BINS, BINS, 0, 0, 0};
     if (x.top_k || x.by_mass) cut = sample_cuts<PIECE_THREADS>(a, x, s);
     const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
-    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t) {
+    if (tid == 0) {
+        held = 0;
+        sum = 0;
+    }
+    __syncthreads();
+    const int end = min(a.tiles, (piece + 1) * a.per);
+    for (int t = piece * a.per; t < end; ++t) {
         uint64_t mine = 0;
-        if (tid == 0) sum = 0;
         tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
 #pragma unroll
             for (int e = 0; e < Chunk<T>::E; ++e) {
@@ -458,28 +494,37 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
                     const double w = x.weight(c.x[e]);
                     if (w >= x.min_p || i + e == x.at) mine += x.fixed(w);
                 }
-                const bool look = real && b >= cut.lo && (b <= cut.hi || b == cut.k);
-                const uint64_t who = __ballot(look);
-                if (who) {                                            // the wave's tokens, side by side
-                    uint32_t at = 0;
-                    const int leader = __builtin_ctzll(who);
-                    if (lane == leader) at = atomicAdd(&a.length[s], (uint32_t)__popcll(who));
-                    at = __shfl(at, leader, WAVE) + __popcll(who & ((1ull << lane) - 1));
-                    if (look && at < LIST) a.list[s * LIST + at] = uint2{(uint32_t)(i + e), order_key(c.x[e])};
-                }
+                if (real && b >= cut.lo && (b <= cut.hi || b == cut.k))
+                    gather[atomicAdd(&held, 1u)] = uint2{(uint32_t)(i + e), order_key(c.x[e])};
             }
         });
+        if (cut.lo > 0) {
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) mine += __shfl_xor(mine, m, WAVE);
+            for (int m = 32; m >= 1; m >>= 1) mine += __shfl_xor(mine, m, WAVE);
+            if (lane == 0 && mine) atomicAdd(&sum, (unsigned long long)mine);
+        }
         __syncthreads();
-        if (lane == 0 && mine) atomicAdd(&sum, (unsigned long long)mine);
+        const uint32_t n = held;
+        const bool flush = n > 0 && (n > GATHER - TILE || t + 1 == end);
         __syncthreads();
-        if (tid == 0) a.sums[s * a.tiles + t] = sum;
+        if (tid == 0) {
+            a.sums[s * a.tiles + t] = sum;
+            sum = 0;
+            if (flush) {
+                place = atomicAdd(&a.length[s], n);
+                held = 0;
+            }
+        }
         __syncthreads();
+        if (flush) {
+            for (uint32_t i = tid; i < n; i += PIECE_THREADS)
+                if (place + i < LIST) a.list[s * LIST + place + i] = gather[i];
+            __syncthreads();
+        }
     }
 }
 
-constexpr int TOKEN_THREADS = 1024, MAX_TILES = (1 << 24) / TILE;
+constexpr int TOKEN_THREADS = 256, MAX_TILES = (1 << 24) / TILE;
 
 // The order as one number, larger first: the key, then the smaller index
 __device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
@@ -508,14 +553,18 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         const SampleCuts cut = sample_cuts<TOKEN_THREADS>(a, x, s);
         lo = cut.lo;
         if (n <= LIST) {
-            // sorted, the largest first (bitonic; the places behind the list hold 0, below every token)
+            // sorted, the largest first (bitonic; the places behind the list hold 0, below every token). Up to a distance of
+            // 64 a wave's pairs lie in 128 places of its own, and its LDS operations stay in order: no barrier
             int size = 2;
             while (size < n) size <<= 1;
             for (int i = tid; i < size; i += TOKEN_THREADS)
                 list[i] = i < n ? order_of(a.list[s * LIST + i].y, a.list[s * LIST + i].x) : 0;
-            __syncthreads();
+            bool apart = true;
             for (int k = 2; k <= size; k <<= 1)
                 for (int j = k >> 1; j > 0; j >>= 1) {
+                    if (apart || j > 64) __syncthreads();
+                    asm volatile("" ::: "memory");
+                    apart = j > 64;
                     for (int i = tid; i < size / 2; i += TOKEN_THREADS) {
                         const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1)), q = p | j;
                         const uint64_t u = list[p], v = list[q];
@@ -524,13 +573,10 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
                             list[q] = u;
                         }
                     }
-                    __syncthreads();
                 }
-            // each thread a run of the sorted list; weights in registers
-            const int run = (size + TOKEN_THREADS - 1) / TOKEN_THREADS;          // LIST / TOKEN_THREADS at most
-            uint64_t m[LIST / TOKEN_THREADS], mine = 0, in_k = 0;
+            __syncthreads();
             const auto token = [&](int i) { return key_logit((uint32_t)(list[i] >> 32)); };
-            // of class k, the first top_k - above_k tokens: their mass makes the kept mass exact
+            // of class k, the first top_k - above_k tokens
             int k_first = n;
             if (x.top_k) {
                 if (tid == 0) shared_at = n;
@@ -540,45 +586,46 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
                 __syncthreads();
                 k_first = shared_at;
             }
-            const int k_end = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : n;     // the list's tokens up to top-k's cut
-#pragma unroll
-            for (int e = 0; e < LIST / TOKEN_THREADS; ++e) {
-                const int i = tid * run + e;
-                m[e] = e < run && i < n && x.by_mass ? x.fixed(x.weight(token(i))) : 0;
-                mine += m[e];
-                if (i >= k_first && i < k_end) in_k += m[e];
-            }
-            int keep = k_end;
+            int keep = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : n;              // the list's tokens up to top-k's cut
+            double limit = 0.0;
             if (x.by_mass) {
-                uint64_t all, k_mass;
-                uint64_t before = block_scan<TOKEN_THREADS>(mine, part, all) - mine + cut.before_lo;
-                block_scan<TOKEN_THREADS>(in_k, part, k_mass);
-                uint64_t total = cut.before_k + k_mass;
-                if (!x.top_k) {                                    // the mass of the row
-                    uint64_t sum = 0;
+                // the mass that top-k keeps: below the list's classes, and its own tokens (bin_mass false: the list starts at
+                // the first token); without top-k all of the row's
+                uint64_t sum = 0, total;
+                if (x.top_k)
+                    for (int i = (x.bin_mass ? k_first : 0) + tid; i < keep; i += TOKEN_THREADS) sum += x.fixed(x.weight(token(i)));
+                else
                     for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
-                    block_scan<TOKEN_THREADS>(sum, part, total);
-                }
-                const double limit = mass_limit(x, total);
-                int here = 0;
-#pragma unroll
-                for (int e = 0; e < LIST / TOKEN_THREADS; ++e) {
-                    const int i = tid * run + e;
-                    if (e < run && i < n) here += (double)before < limit;
-                    before += m[e];
-                }
-                int kept_all;
-                block_scan<TOKEN_THREADS>(here, reinterpret_cast<int*>(part), kept_all);
-                keep = min(keep, kept_all);
+                block_scan<TOKEN_THREADS>(sum, part, total);
+                limit = mass_limit(x, x.top_k ? cut.before_k + total : total);
             }
-            least = keep > 0 ? list[keep - 1] : ~0ull;
-            // the kept tokens' mass to their tiles
-            __syncthreads();
-            for (int i = tid; i < keep; i += TOKEN_THREADS) {
-                const double w = x.weight(token(i));
-                const uint32_t at = ~(uint32_t)list[i];
-                if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)x.fixed(w));
+            // the tokens that are kept: their mass to their tiles
+            uint64_t before = cut.before_lo;
+            int kept = 0;
+#pragma unroll 1
+            for (int i0 = 0; i0 < keep; i0 += TOKEN_THREADS) {
+                const int i = i0 + tid;
+                double w = 0.0;
+                uint64_t m = 0, all = 0;
+                if (i < keep) {
+                    w = x.weight(token(i));
+                    m = x.fixed(w);
+                }
+                bool mine = i < keep;
+                if (x.by_mass) {
+                    const uint64_t run = before + block_scan<TOKEN_THREADS>(m, part, all) - m;
+                    before += all;
+                    mine = mine && (double)run < limit;
+                }
+                if (mine) {
+                    const uint32_t at = ~(uint32_t)list[i];
+                    if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)m);
+                }
+                const int now = __syncthreads_count(mine);
+                kept += now;
+                if (now < TOKEN_THREADS) break;
             }
+            least = kept > 0 ? list[kept - 1] : ~0ull;
         } else {
             // the token that ends what is kept, by a radix search over the row's orders: 11 bits a pass, from the top
             uint64_t* const mass = list;
@@ -661,11 +708,10 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     __syncthreads();
     // the tile that the target falls into
     uint64_t run_mass = 0, all = 0;
-    for (int t0 = 0; t0 < a.tiles; t0 += TOKEN_THREADS) {
-        uint64_t here;
-        const uint64_t v = t0 + tid < a.tiles ? (uint64_t)sums[t0 + tid] : 0;
-        block_scan<TOKEN_THREADS>(v, part, here);
-        all += here;
+    {
+        uint64_t v = 0;
+        for (int t = tid; t < a.tiles; t += TOKEN_THREADS) v += sums[t];
+        block_scan<TOKEN_THREADS>(v, part, all);
     }
     // (a random number of 1 or more: the last kept token)
     const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
@@ -688,26 +734,32 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         if (tid == 0) a.out[r] = x.at;
         return;
     }
-    constexpr int E = TILE / TOKEN_THREADS;
-    uint64_t m[E], mine = 0, unused;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
+    // each thread a run of the tile's tokens, from LDS (a run and a bit apart, so that the threads read different banks)
+    constexpr int E = TILE / TOKEN_THREADS, RUN = E + 1;
+    float* const logit = reinterpret_cast<float*>(list);
+    for (int i = tid; i < TILE; i += TOKEN_THREADS)
+        logit[i / E * RUN + i % E] = tile * TILE + i < a.vocab ? to_f32(row[tile * TILE + i]) : -__builtin_inff();
+    __syncthreads();
+    const auto mass_at = [&](int e) -> uint64_t {
         const int i = tile * TILE + tid * E + e;
-        m[e] = 0;
-        if (i < a.vocab) {
-            const float v = to_f32(row[i]);
-            if (x.bin(v) < lo || order_of(order_key(v), i) >= least) {
-                const double w = x.weight(v);
-                if (w >= x.min_p || i == x.at) m[e] = x.fixed(w);
+        const float v = logit[tid * RUN + e];
+        if (i >= a.vocab || !(x.bin(v) < lo || order_of(order_key(v), i) >= least)) return 0;
+        const double w = x.weight(v);
+        return w >= x.min_p || i == x.at ? x.fixed(w) : 0;
+    };
+    uint64_t mine = 0, unused;
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) mine += mass_at(e);
+    uint64_t before = run_mass + block_scan<TOKEN_THREADS>(mine, part, unused) - mine;
+    if (mine && (double)before <= want && (double)(before + mine) > want) {
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+            before += mass_at(e);
+            if ((double)before > want) {
+                a.out[r] = tile * TILE + tid * E + e;
+                break;
             }
         }
-        mine += m[e];
-    }
-    uint64_t before = run_mass + block_scan<TOKEN_THREADS>(mine, part, unused) - mine;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (m[e] && (double)before <= want && (double)(before + m[e]) > want) a.out[r] = tile * TILE + tid * E + e;
-        before += m[e];
     }
 }
 

@@ -168,7 +168,7 @@ PyObject* decode(PyObject* const* a) {
     void* const stream = (void*)integer(a[24], 0, INT64_MAX);
     CALL("kush_window_decode",
          g_decode(D, bits, G, dtype, pq, pout, pc, bs, hs, pt, ptix, ptab, plen, row, H, scale, ns, ml, po, S, stream, pk, pv,
-                  ks, vs, sync, waves, order, rot, window, sinks));
+                  ks, vs, (int32_t)std::min<int64_t>(table.size(1), 1 << 30), sync, waves, order, rot, window, sinks));
     Py_RETURN_TRUE;
 }
 
