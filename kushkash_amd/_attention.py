@@ -248,7 +248,7 @@ def _unpacked_rows(ops, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.T
         tail_blk = block_table[:, full].contiguous()
         first = first_rows(full * PAGE, full * PAGE + 1, 1)
         info = torch.stack([first, torch.full_like(first, n_hist % PAGE), tail_idx[:B].to(torch.int32)], dim=1).view(-1)
-    ops.unpack(cache, block_table[:, :full].reshape(-1), first_rows(0, full * PAGE, PAGE), tail_blk, info, tail_k, *new,
+    ops.unpack(cache, block_table[:, :full].reshape(-1).contiguous(), first_rows(0, full * PAGE, PAGE), tail_blk, info, tail_k, *new,
                first_rows(n_hist, rows, 1), kp.view(-1, Hk, D), vp.view(-1, Hk, D), rot)
     return kp, vp
 
