@@ -627,9 +627,12 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
             }
             least = kept > 0 ? list[kept - 1] : ~0ull;
         } else {
-            // the token that ends what is kept, by a radix search over the row's orders: 11 bits a pass, from the top
+            // the token that ends what is kept, by a radix search over the row's orders: 9 bits a pass, from the top,
+            // two bins to a thread
+            constexpr int SEARCH = 9;
+            static_assert((1 << SEARCH) == 2 * TOKEN_THREADS, "two bins to a thread");
             uint64_t* const mass = list;
-            uint32_t* const count = reinterpret_cast<uint32_t*>(list + 2048);
+            uint32_t* const count = reinterpret_cast<uint32_t*>(list + (1 << SEARCH));
             const auto each = [&](auto&& fn) {
                 for (int i = tid; i < a.vocab; i += TOKEN_THREADS) fn(i, to_f32(row[i]));
             };
@@ -638,9 +641,9 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
             const auto search = [&](bool by_mass, uint64_t floor, uint32_t want, double limit, uint64_t& kept) -> uint64_t {
                 uint64_t prefix = 0, above_mass = 0, above = 0;
                 for (int top = 64; top > 0;) {
-                    const int width = min(11, top), shift = top - width, nb = 1 << width;
+                    const int width = min(SEARCH, top), shift = top - width, nb = 1 << width;
                     __syncthreads();
-                    for (int i = tid; i < 2048; i += TOKEN_THREADS) {
+                    for (int i = tid; i < (1 << SEARCH); i += TOKEN_THREADS) {
                         mass[i] = 0;
                         count[i] = 0;
                     }
