@@ -26,6 +26,7 @@ from functools import lru_cache
 import torch
 
 from . import _attend
+from ._window import window_attention
 from ._records import PAGE, as_records, dequant_records
 
 
@@ -251,6 +252,25 @@ def _unpacked_rows(ops, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.T
     ops.unpack(cache, block_table[:, :full].reshape(-1).contiguous(), first_rows(0, full * PAGE, PAGE), tail_blk, info, tail_k, *new,
                first_rows(n_hist, rows, 1), kp.view(-1, Hk, D), vp.view(-1, Hk, D), rot)
     return kp, vp
+
+
+def windowed_history_attention(ops, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.Tensor, maps,
+                               tail_k: torch.Tensor, scale: float, rot: bool, window: int, sinks: int) -> torch.Tensor:
+    """Attention of a chunk of T queries over a cached history and the chunk itself under a window: the history's pages
+    that maps (step_maps with the window; None: no history) keep are unpacked with the chunk's rows behind them by one
+    launch, and window_attention runs over the rows, in the cache's dtype. Shapes as history_attention; returns q's dtype."""
+    B, Hk, T, D = k_new.shape
+    if maps is None:
+        rows = [x.transpose(1, 2) for x in (q, k_new, v_new)]
+        return window_attention(*rows, window=window, sinks=sinks, scale=scale).transpose(1, 2)
+    new = [x.to(ops.dtype).transpose(1, 2).reshape(B * T, Hk, D) for x in (k_new, v_new)]
+    new = [x if x.stride(2) == 1 and x.stride(1) == D else x.contiguous() for x in new]
+    kp, vp = (torch.empty(maps.sizes.keys, Hk, D, dtype=ops.dtype, device=k_new.device) for _ in range(2))
+    ops.unpack(cache, maps.page_blk, maps.page_dst, maps.tail_blk, maps.tail_info.view(-1), tail_k, *new, maps.new_dst, kp, vp,
+               rot)
+    out = window_attention(q.to(ops.dtype).transpose(1, 2), kp.view(B, -1, Hk, D), vp.view(B, -1, Hk, D), window=window,
+                           sinks=sinks, scale=scale)
+    return out.transpose(1, 2).to(q.dtype)
 
 
 def unpacked_history_attention(ops, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.Tensor,

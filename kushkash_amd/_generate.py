@@ -16,17 +16,23 @@ import time
 
 import torch
 
+from ._step import sample
 from .hf import NAME, KushHFCache, enable
 
 WARMUP_STEPS = 2      # eager steps (on a side stream, as torch's capture asks) before the capture
 EOS_LAG = 2           # the host reads a step's EOS flags this many steps after queuing it
 
 
-def _pick(logits: torch.Tensor, do_sample: bool, temperature: float, top_k: int) -> torch.Tensor:
+def _pick(logits: torch.Tensor, do_sample: bool, temperature: float, top_k: int, top_p: float = 1.0, min_p: float = 0.0,
+          generator: torch.Generator | None = None) -> torch.Tensor:
     """Next token per row: argmax, or a sample from softmax(logits / temperature) restricted to the
-    top_k largest logits when top_k > 0 (_generate.py:23-30)."""
+    top_k largest logits when top_k > 0 (_generate.py:23-30). With top_p, min_p or a generator: by the sampling kernel
+    (kushkash_amd.sample) from one random number per row."""
     if not do_sample:
         return logits.argmax(-1)
+    if generator is not None or top_p < 1.0 or min_p > 0.0:
+        u = torch.rand(logits.shape[0], dtype=torch.float32, device=logits.device, generator=generator)
+        return sample(logits, u, temperature=max(temperature, 1e-5), top_k=top_k, top_p=top_p, min_p=min_p)
     z = logits.float() / max(temperature, 1e-5)
     if top_k:
         top = z.topk(min(top_k, z.shape[-1]), dim=-1)
@@ -146,7 +152,9 @@ class _DecodeStep:
 def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int = 4,
              cache: KushHFCache | None = None, prefill_chunk: int = 1024, cuda_graph: bool | str = "auto",
              eos_token_id: int | list[int] | None = None, do_sample: bool = False,
-             temperature: float = 1.0, top_k: int = 0, stats: dict | None = None) -> torch.Tensor:
+             temperature: float = 1.0, top_k: int = 0, stats: dict | None = None, top_p: float = 1.0,
+             min_p: float = 0.0, generator: torch.Generator | None = None, window: int | str | None = None,
+             sinks: int = 0) -> torch.Tensor:
     """[B, prompt + generated] token ids; rows that reach EOS are padded with EOS.
 
     Args:
@@ -156,15 +164,24 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
             > 10 % faster than an eager step), True (always), False (never).
         stats: optional dict, filled with prefill_s, prefill_history_attn_s, decode_s, decode_tokens,
             graph, eager_step_ms, graph_step_ms.
+        do_sample, temperature, top_k, top_p, min_p: sample (kushkash_amd.sample has their meaning); generator: where the
+            random numbers come from (None: torch's own of the device).
+        window, sinks: what a query sees of the tokens up to its own (KushHFCache's options): the last `window` and the
+            first `sinks`; "config" takes a sliding-window model's own windows. A cache that is given brings its own.
     """
+    if cache is not None and (window is not None or sinks):
+        raise ValueError("window and sinks are the cache's: build it with them, or pass none")
+    if not 0.0 <= top_p or not 0.0 <= min_p:
+        raise ValueError(f"top_p and min_p must be >= 0, got {top_p} and {min_p}")
     if model.config._attn_implementation != NAME:
-        enable(model)
+        enable(model, sliding_window=window == "config")
     dev = input_ids.device
     if dev.type != "cuda":
         raise ValueError("kushkash_amd.generate runs on the GPU (input_ids on a 'cuda' device under ROCm)")
     B, T0 = input_ids.shape
     total = T0 + max_new_tokens
-    cache = cache if cache is not None else KushHFCache(model.config, bits=bits, max_length=total)
+    cache = cache if cache is not None else KushHFCache(model.config, bits=bits, max_length=total, window=window,
+                                                               sinks=sinks)
     eos_ids = [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id or [])
     stop = _StopSignal(torch.tensor(eos_ids, dtype=torch.long, device=dev), B, dev) if eos_ids else None
 
@@ -178,7 +195,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
             cache.kv.profile = []               # time the chunks that attend over history
         ids = input_ids[:, c0:c0 + prefill_chunk]
         logits = forward(ids, torch.arange(c0, c0 + ids.shape[1], device=dev).expand(B, -1))
-    tok = _pick(logits, do_sample, temperature, top_k)
+    pick = (do_sample, temperature, top_k, top_p, min_p, generator)
+    tok = _pick(logits, *pick)
     torch.cuda.synchronize(dev)
     t1 = time.perf_counter()
 
@@ -189,7 +207,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
     for i in range(1, max_new_tokens):
         if stop is not None and stop.finished(tok, i):
             break
-        tok = _pick(step(tok, T0 + i - 1), do_sample, temperature, top_k)
+        tok = _pick(step(tok, T0 + i - 1), *pick)
         if stop is not None:
             tok = stop.mask(tok)
         out.append(tok)

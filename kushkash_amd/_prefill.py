@@ -8,7 +8,8 @@ kushkash/vllm/backend.py:385-475, :807-880.
 Host side, once per step (``ExtendPlan``): the write jobs (one per (request, logical page) the new
 tokens touch), and the attention groups: consecutive requests whose K + V, history and new tokens
 together, fit a byte budget are packed end to end; a request over the budget alone (and every request
-in loop mode) takes its history in blocks of pages. All index arrays go to the device in one copy.
+in loop mode) takes its history in blocks of pages. The lengths and tail slots go to the device in one copy;
+every index array is built from them there (_step.step_maps).
 
 Device side, per layer (``ExtendPlan.attend``, before the step's write): per packed group one launch of
 the unpack kernel builds every request's keys [history pages | partial page (K from the tail, V from
@@ -27,8 +28,9 @@ import numpy as np
 import torch
 
 from ._attention import ragged_attention, unpacked_history_attention
-from ._ops import PAGE, pages_touched
+from ._ops import PAGE
 from ._serving import torch_unpack, unpack_mode
+from ._step import map_sizes, step_maps
 
 
 def record_bits() -> int:
@@ -150,45 +152,36 @@ class ExtendPlan:
     @classmethod
     def build(cls, new_tokens, history, slots, block_table: torch.Tensor, *, kv_heads: int, head_dim: int,
               dtype: torch.dtype, packed: bool = True, budget: int | None = None, upload=None) -> "ExtendPlan":
-        """upload(int32 numpy array) -> device tensor: how the step's one host -> device copy is made
-        (default: a plain copy to the block table's device)."""
+        """upload(int32 numpy array) -> device tensor: how the step's one host -> device copy (its lengths and slots) is
+        made (default: a plain copy to the block table's device)."""
         q = np.asarray(new_tokens, dtype=np.int64)
         h = np.asarray(history, dtype=np.int64)
         slots = np.asarray(slots, dtype=np.int64)
         total = h + q
+        R = len(q)
         q_start = np.concatenate([[0], np.cumsum(q)])
-        jobs = [(r, p) for r in range(len(q)) for p in pages_touched(int(h[r]), int(total[r]))]
-        job_arr = np.asarray(jobs, dtype=np.int64).reshape(-1, 2)
         elem = torch.empty((), dtype=dtype).element_size()
         layout = group_requests(q, h, 2 * kv_heads * head_dim * elem, pack_budget() if budget is None else budget,
                                 packed)
-        host = [q_start, job_arr[:, 0], job_arr[:, 1]]
-        plans = []
-        for r0, r1, is_packed in layout:
-            if not is_packed:
-                plans.append(None)
-                continue
-            p = pack_plan(q[r0:r1], h[r0:r1], slots[r0:r1])
-            plans.append(p)
-            host += [p.key_start, q_start[r0:r1 + 1] - q_start[r0], r0 + p.page_req, p.page_index, p.page_dst,
-                     r0 + p.tail_req, h[r0 + p.tail_req] // PAGE, p.tail_info.reshape(-1), p.new_dst]
-        flat = np.concatenate(host).astype(np.int32)
-        dev = (upload or (lambda a: _host_to_device(a, block_table.device)))(flat)
-        views, at = [], 0
-        for a in host:
-            views.append(dev[at:at + len(a)])
-            at += len(a)
-        plan = cls(views[0], views[1], views[2], q_start_host=[int(x) for x in q_start],
+        # the lengths and slots go over; every index array is built from them on the device
+        lens = np.concatenate([q, h, slots]).astype(np.int32)
+        dev = (upload or (lambda a: _host_to_device(a, block_table.device)))(lens)
+        parts = dev[:R], dev[R:2 * R], dev[2 * R:3 * R]
+
+        def maps(r0, r1, writes):
+            sizes = map_sizes(q[r0:r1].tolist(), h[r0:r1].tolist())
+            return step_maps(*(x[r0:r1] for x in parts), block_table[r0:r1], sizes.writes() if writes else sizes)
+
+        whole = maps(0, R, writes=len(layout) != 1 or not layout[0][2])
+        plan = cls(whole.q_start, whole.job_seq, whole.job_page, q_start_host=[int(x) for x in q_start],
                    history_host=[int(x) for x in h])
-        rest = iter(views[3:])
-        for (r0, r1, is_packed), p in zip(layout, plans):
+        for r0, r1, is_packed in layout:
             g = Group(r0, r1, is_packed)
-            if p is not None:
-                g.cu_k, g.cu_q, page_req, page_index, g.page_dst, tail_req, tail_page, g.tail_info, g.new_dst = (
-                    next(rest) for _ in range(9))
-                g.page_blk = block_table[page_req.long(), page_index.long()].contiguous()
-                g.tail_blk = block_table[tail_req.long(), tail_page.long()].contiguous()
-                g.key_start = [int(x) for x in p.key_start]
+            if is_packed:
+                m = whole if (r0, r1) == (0, R) else maps(r0, r1, writes=False)
+                g.cu_k, g.cu_q, g.page_blk, g.page_dst = m.key_start, m.q_start, m.page_blk, m.page_dst
+                g.tail_blk, g.tail_info, g.new_dst = m.tail_blk, m.tail_info.view(-1), m.new_dst
+                g.key_start = [0, *(int(x) for x in np.cumsum(total[r0:r1]))]
                 g.n_keys = g.key_start[-1]
                 g.has_history = bool(h[r0:r1].any())
                 g.max_q = int(q[r0:r1].max())

@@ -4,7 +4,7 @@ tokens, drawn from the logits and given random numbers. On other devices block_t
 of the same results (what the serving integrations' host path runs on); sample is for the GPU."""
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
@@ -98,6 +98,10 @@ class MapSizes:
         object.__setattr__(self, "numbers", (self.requests, self.tokens, self.keys, self.jobs, self.pages, self.tails,
                                              self.window, self.sinks))
 
+    def writes(self) -> "MapSizes":
+        """The sizes without the maps that unpack history: of a step that only writes its tokens."""
+        return replace(self, pages=0, tails=0)
+
 
 @dataclass
 class StepMaps:
@@ -113,6 +117,7 @@ class StepMaps:
     tail_info: torch.Tensor    # [tails, 3]   its first key row, tokens and tail slot
     new_dst: torch.Tensor      # [tokens] key row of every new token
     slot_map: torch.Tensor     # [tokens] its block * 32 + its row in the page
+    sizes: MapSizes
 
 
 def map_sizes(new_tokens, history, *, window: int | None = None, sinks: int = 0) -> MapSizes:
@@ -145,7 +150,7 @@ def step_maps(new_tokens: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     ragged attention of the step take. sizes: map_sizes of the same lengths, which the host knows before the step. Lengths
     on the device that need more than the sizes hold are cut off at them."""
     if new_tokens.is_cuda and (got := _native("step_maps", new_tokens, history, slots, block_table, sizes.numbers)) is not None:
-        return StepMaps(*got)
+        return StepMaps(*got, sizes)
     dev, R = new_tokens.device, sizes.requests
     for name, t in (("new_tokens", new_tokens), ("history", history), ("slots", slots)):
         _index(name, t, R, dev)
@@ -158,7 +163,7 @@ def step_maps(new_tokens: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     at += at & 1                                                    # the int64 map behind them, 8-byte aligned
     buf = torch.empty(at + 2 * sizes.tokens, dtype=torch.int32, device=dev)
     maps = StepMaps(**{name: buf[a:a + n].view(-1, 3) if width == 3 else buf[a:a + n] for name, a, n, width in cuts},
-                    slot_map=buf[at:].view(torch.int64))
+                    slot_map=buf[at:].view(torch.int64), sizes=sizes)
     if R == 0:
         buf.zero_()
     elif dev.type != "cuda":
@@ -188,10 +193,10 @@ def _host_maps(m: StepMaps, new_tokens, history, slots, block_table, sizes: MapS
     r, i = runs(torch.where(t > 0, (h + t - 1) // PAGE - full + 1, 0))
     m.job_seq.copy_(r)
     m.job_page.copy_(full[r] + i)
-    r, i = runs(full - gap)
+    r, i = (x[:sizes.pages] for x in runs(full - gap))
     m.page_blk.copy_(block_table[r, torch.where(i < first, i, i + gap[r])])
     m.page_dst.copy_(m.key_start[r] + PAGE * i)
-    r, _ = runs((h % PAGE > 0).long())
+    r = runs((h % PAGE > 0).long())[0][:sizes.tails]
     m.tail_blk.copy_(block_table[r, full[r]])
     m.tail_info.copy_(torch.stack([m.key_start[r] + PAGE * (full - gap)[r], h[r] % PAGE, slots[r].long()], 1))
     r, i = runs(t)

@@ -27,10 +27,12 @@ from dataclasses import dataclass
 
 import torch
 
-from ._attention import unpacked_history_attention
-from ._ops import PAGE, Ops, default_scale, pages_touched, record_bytes
+from ._attention import unpacked_history_attention, windowed_history_attention
+from ._ops import PAGE, Ops, default_scale, record_bytes
 from ._records import cached_kv
 from ._rotation import hadamard, rotate, rotation_enabled
+from ._step import map_sizes, step_maps
+from ._window import check_limit
 
 _KERNEL_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -68,12 +70,16 @@ class KushCache:
         rotate_in_kernels: with rotation on, let the kernels rotate (canonical Walsh-Hadamard
             transform) instead of a torch product around them; no counterpart in the reference, the
             stored values differ from the product's only in rounding.
+        window, sinks: what a query sees of the tokens up to its own: the last `window` and the first `sinks` (None: all
+            of them). window may be a sequence with one entry per layer. On the GPU; no counterpart in the reference.
+            Every token is kept, so memory is the same; what a step reads is bounded.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, num_q_heads: int, head_dim: int, *,
                  batch_size: int = 1, bits: int = 4, device: str | torch.device = "cuda",
                  dtype: torch.dtype = torch.float16, max_length: int | None = None, scale: float | None = None,
-                 rotate: bool | None = None, rotate_in_kernels: bool = False):
+                 rotate: bool | None = None, rotate_in_kernels: bool = False,
+                 window: int | None | list[int | None] = None, sinks: int = 0):
         if bits not in (4, 8):
             raise ValueError("bits must be 4 or 8")
         if num_kv_heads < 1 or num_q_heads % num_kv_heads:
@@ -97,6 +103,15 @@ class KushCache:
         if rotate_in_kernels and not self.gpu:
             raise ValueError("rotate_in_kernels is for the GPU kernels; on the CPU the cache rotates with torch")
         self.krot = self.rot is not None and bool(rotate_in_kernels)
+        windows = list(window) if isinstance(window, (list, tuple)) else [window] * num_layers
+        if len(windows) != num_layers:
+            raise ValueError(f"window must be one for all layers or one per layer ({num_layers}), got {len(windows)}")
+        if sinks and all(w is None for w in windows):
+            check_limit(None, sinks)
+        # per layer (window, sinks), (0, 0): none
+        self._limits = [check_limit(w, 0 if w is None else sinks) for w in windows]
+        if not self.gpu and any(w for w, _ in self._limits):
+            raise ValueError("a window is for the GPU kernels; on the CPU the cache attends over every token")
         self.profile: list | None = None                          # a list: attend_chunk records event pairs
         self.tail_k = torch.zeros(num_layers, batch_size, num_kv_heads, PAGE, head_dim, dtype=self.kdtype,
                                   device=device)
@@ -166,6 +181,10 @@ class KushCache:
         return (x if x.is_contiguous() else x.contiguous()).view(B * T, H, D)
 
     # ---------------------------------------------------------------- writes and attention
+    def layer_limit(self, layer: int) -> tuple[int, int]:
+        """(window, sinks) of a layer; (0, 0) without a window."""
+        return self._limits[layer]
+
     def length(self, layer: int = 0) -> int:
         return self._tokens[layer]
 
@@ -186,15 +205,19 @@ class KushCache:
         if T == 1:
             self.ops.append(kr, vr, self.seq_lens[layer], self.tail_idx, pos_offset=0, advance=True, **dst, **kw)
         else:
-            self.seq_lens[layer].fill_(n + T)
-            touched = pages_touched(n, n + T)
-            pages = torch.arange(touched.start, touched.stop, dtype=torch.int32, device=self.device)
-            seqs = torch.arange(B, dtype=torch.int32, device=self.device)
-            starts = seqs * T
-            qsl = torch.cat([starts, starts[-1:] + T])
-            self.ops.write(kr, vr, qsl, self.seq_lens[layer], self.tail_idx,
-                           seqs.repeat_interleave(len(touched)), pages.repeat(B), **dst, fused=True, **kw)
+            m = self._maps(n, T, history=False)
+            self.seq_lens[layer].copy_(m.seq_lens)
+            self.ops.write(kr, vr, m.q_start, m.seq_lens, self.tail_idx, m.job_seq, m.job_page, **dst, fused=True, **kw)
         self._tokens[layer] = n + T
+
+    def _maps(self, n: int, T: int, history: bool = True, window: int = 0, sinks: int = 0):
+        """The index arrays of T new tokens per sequence over n cached ones (history: with those that unpack the cached
+        ones that a window leaves): built on the device, as the lengths are."""
+        new, old = (torch.full((self.B,), x, dtype=torch.int32, device=self.device) for x in (T, n))
+        sizes = map_sizes([T] * self.B, [n] * self.B, window=window or None, sinks=sinks)
+        if not history:
+            sizes = sizes.writes()
+        return step_maps(new, old, self.tail_idx, self.block_table, sizes)
 
     def attend(self, layer: int, q: torch.Tensor) -> torch.Tensor:
         """Decode attention of one query per sequence over all its cached tokens. q [B, Hq, D] (q head i
@@ -231,9 +254,15 @@ class KushCache:
         qk = (q.to(self.kdtype) if rot else self._inward(q)).contiguous()
         out = torch.empty_like(qk)
         pages = (self._capacity if self._splits else self._tokens[layer]) // PAGE
-        splits = self._splits or self.ops.splits(self.B, self.H, pages)
-        self._ensure_work(splits)
+        window, sinks = self._limits[layer]
         kw = {"rot": True} if rot else {}
+        if window:
+            kw.update(window=window, sinks=sinks)
+            splits = self.ops.splits(self.B, self.H, pages, window=window, sinks=sinks)
+            pages = min(pages, window // PAGE)
+        else:
+            splits = self._splits or self.ops.splits(self.B, self.H, pages)
+        self._ensure_work(splits)
         if self.gpu:                                     # waves by the cached length (the table is wider)
             kw["waves"] = self.ops.waves(self.B, self.H, splits, pages)
         dst = (self.pool[layer], self.block_table)
@@ -254,14 +283,22 @@ class KushCache:
         before the chunk is written; q [B, Hq, T, D], k, v [B, Hkv, T, D] -> [B, Hq, T, D]
         (cache.py:185-201). The history is unpacked a block of pages at a time by the unpack kernel,
         rotated back in that kernel when the cache rotates, so the attention itself runs on the
-        unrotated q and chunk; extra memory stays within ~block_bytes at any history length."""
+        unrotated q and chunk; extra memory stays within ~block_bytes at any history length. Under a window the
+        history's pages that no query of the chunk sees are not unpacked, and the extra memory is the rest and the chunk."""
         timing = self.profile is not None and q.is_cuda
         if timing:
             ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
             ev[0].record()
-        out = unpacked_history_attention(self.ops, q, k, v, self.pool[layer], self.block_table, self._tokens[layer],
-                                         self.tail_k[layer], self.tail_idx, self.scale, self.rot is not None,
-                                         block_bytes)
+        window, sinks = self._limits[layer]
+        if window:
+            n = self._tokens[layer]
+            out = windowed_history_attention(self.ops, q, k, v, self.pool[layer], self._maps(n, q.shape[2], window=window,
+                                             sinks=sinks) if n else None, self.tail_k[layer], self.scale,
+                                             self.rot is not None, window, sinks)
+        else:
+            out = unpacked_history_attention(self.ops, q, k, v, self.pool[layer], self.block_table, self._tokens[layer],
+                                             self.tail_k[layer], self.tail_idx, self.scale, self.rot is not None,
+                                             block_bytes)
         if timing:
             ev[1].record()
             self.profile.append(ev)
@@ -282,7 +319,8 @@ class KushCache:
             raise RuntimeError("freeze() is for the GPU path")
         self._reserve(-(-max_tokens // PAGE))
         self._splits = self.ops.splits(self.B, self.H, max_tokens // PAGE)
-        self._ensure_work(self._splits)
+        self._ensure_work(max([self._splits] + [self.ops.splits(self.B, self.H, max_tokens // PAGE, window=w, sinks=s)
+                                                for w, s in set(self._limits) if w]))
         self._capacity = max_tokens
 
     def advance(self, steps: int = 1) -> None:

@@ -27,6 +27,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import _attend
 from ._attention import self_attention_blocks
+from ._window import window_attention
 from .cache import KushCache
 
 NAME = "kushkash"
@@ -98,17 +99,24 @@ class KushHFCache(Cache):
         max_length: per-sequence capacity to reserve (the pool grows on demand otherwise).
         rotate: Hadamard rotation inside the cache (None: KUSHKASH_ROTATE; auto = on for 4-bit).
         rotate_in_kernels: let the kernels do that rotation (KushCache's option; no reference counterpart).
+        window, sinks: what a query sees of the tokens up to its own: the last `window` and the first `sinks`
+            (KushCache's option; no reference counterpart). None: all of them. "config": each layer's window from the
+            config, for a sliding-window model (enable(model, sliding_window=True)).
     The KushCache is created by the first update(), with the batch size, device and dtype of the
     model's keys (a GPU device: the kernels run on the GPU only).
     """
 
     def __init__(self, config, bits: int = 4, max_length: int | None = None, rotate: bool | None = None,
-                 rotate_in_kernels: bool = False):
+                 rotate_in_kernels: bool = False, window: int | str | None = None, sinks: int = 0):
         cfg = _text_config(config)
         self.num_layers = cfg.num_hidden_layers
         self.num_q_heads = cfg.num_attention_heads
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.bits, self.max_length, self.rotate, self.rotate_in_kernels = bits, max_length, rotate, rotate_in_kernels
+        if isinstance(window, str) and window != "config":
+            raise ValueError(f"window must be a number of tokens, None or 'config', got {window!r}")
+        self.windows = layer_windows(cfg) if window == "config" else [window] * self.num_layers
+        self.sinks = sinks
         self.kv: KushCache | None = None
         super().__init__(layers=[_PagedLayer(self, i) for i in range(self.num_layers)])
 
@@ -122,7 +130,8 @@ class KushHFCache(Cache):
             B, H, _, D = key_states.shape
             self.kv = KushCache(self.num_layers, H, self.num_q_heads, D, batch_size=B, bits=self.bits,
                                 device=key_states.device, dtype=key_states.dtype, max_length=self.max_length,
-                                rotate=self.rotate, rotate_in_kernels=self.rotate_in_kernels)
+                                rotate=self.rotate, rotate_in_kernels=self.rotate_in_kernels, window=self.windows,
+                                sinks=self.sinks if any(self.windows) else 0)
         self.layers[layer_idx].is_initialized = True
         setattr(key_states, _ROUTE, (self, layer_idx))
         return key_states, value_states
@@ -133,7 +142,7 @@ class KushHFCache(Cache):
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
-                     block_bytes: int = 1 << 28) -> torch.Tensor:
+                     block_bytes: int = 1 << 28, *, window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """Causal attention of a prompt over itself when nothing is cached yet: q [B, Hq, T, D], k, v
     [B, Hkv, T, D] -> [B, Hq, T, D] in q's dtype (hf.py:122-129). Half-precision inputs go to the prefill
     attention kernel; what it does not take (rows not 16-byte aligned, derivatives) to torch's fused
@@ -141,7 +150,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     the flash kernel refuses, to fp32 products over blocks of keys whose memory stays within block_bytes.
     torch's memory-efficient kernel is not allowed: on ROCm its dense and varlen forms are the same kernel
     family, and its varlen form with a bottom-right causal mask has taken an illegal-address fault on this
-    device. torch's half-precision math path (batched products over transposed views) is never taken either."""
+    device. torch's half-precision math path (batched products over transposed views) is never taken either.
+    window, sinks: what a query sees of the tokens up to its own (window_attention)."""
+    if window is not None:
+        return window_attention(*(x.transpose(1, 2) for x in (q, k, v)), window=window, sinks=sinks,
+                                scale=scale).transpose(1, 2)
     rows = [x.transpose(1, 2) for x in (q, k, v)]
     if k.shape[2] == q.shape[2] and _attend.takes(*rows, scale):     # else query t sees keys 0 .. t all the same
         return _attend.attend(*rows, True, scale, scratch=block_bytes).transpose(1, 2)
@@ -183,6 +196,11 @@ def kush_attention(module, query, key, value, attention_mask, scaling=None, drop
     kv, layer = route[0].kv, route[1]
     if scaling is not None:
         kv.scale = float(scaling)
+    limit = kv.layer_limit(layer)
+    sliding = kwargs.get("sliding_window")
+    if sliding and not 0 < limit[0] <= sliding and _window_can_bind(_text_config(module.config)):
+        raise RuntimeError(f"kushkash: layer {layer} has a sliding window of {sliding} tokens, its cache "
+                           f"{limit[0] or 'none'}: pass KushHFCache(..., window='config')")
     T = query.shape[2]
     if T == 1:
         return kv.append_attend(layer, query[:, :, 0], key, value).unsqueeze(1), None
@@ -191,7 +209,7 @@ def kush_attention(module, query, key, value, attention_mask, scaling=None, drop
     if kv.length(layer):
         out = kv.attend_chunk(layer, query, key, value)
     else:
-        out = prompt_attention(query, key, value, kv.scale)
+        out = prompt_attention(query, key, value, kv.scale, window=limit[0] or None, sinks=limit[1])
     kv.write(layer, key, value)
     return out.transpose(1, 2).contiguous(), None
 
@@ -222,6 +240,19 @@ def _window_can_bind(cfg) -> bool:
     return window > 0 and (limit is None or window < limit)
 
 
+def layer_windows(cfg) -> list[int | None]:
+    """Each layer's attention window by a config that _window_can_bind looked at: the sliding_window on its
+    "sliding_attention" layers (on every layer without per-layer types), None on the others. Other kinds of layers are
+    refused."""
+    kinds = getattr(cfg, "layer_types", None) or ["sliding_attention"] * cfg.num_hidden_layers
+    window = getattr(cfg, "sliding_window", None) or None
+    if not _window_can_bind(cfg):
+        return [None] * cfg.num_hidden_layers
+    if any(kind not in ("full_attention", "sliding_attention") for kind in kinds) or len(kinds) != cfg.num_hidden_layers:
+        _refuse(f"a model with layers of {sorted(set(kinds))}")
+    return [window if kind == "sliding_attention" else None for kind in kinds]
+
+
 # (test on the text config, what is refused): attention these kernels do not compute (hf.py:209-216)
 _UNSUPPORTED = (
     (_window_can_bind, "sliding-window / hybrid attention layers"),
@@ -230,10 +261,12 @@ _UNSUPPORTED = (
 )
 
 
-def _check_config(config) -> None:
+def _check_config(config, sliding_window: bool = False) -> None:
     cfg = _text_config(config)
     for test, what in _UNSUPPORTED:
-        if test(cfg):
+        if sliding_window and test is _window_can_bind:
+            layer_windows(cfg)
+        elif test(cfg):
             _refuse(what)
 
 
@@ -242,10 +275,11 @@ def register() -> None:
     AttentionMaskInterface.register(NAME, kush_mask)
 
 
-def enable(model):
+def enable(model, *, sliding_window: bool = False):
     """Check the model's config, register the "kushkash" attention and mask functions and select them;
-    returns the model."""
-    _check_config(model.config)
+    returns the model. sliding_window: take a model whose layers have sliding windows too; its cache is then
+    KushHFCache(..., window="config"), which keeps every token and attends over the windows."""
+    _check_config(model.config, sliding_window)
     register()
     model.set_attn_implementation(NAME)
     return model

@@ -39,6 +39,7 @@ from .._ops import PAGE, Ops
 from .._prefill import ExtendPlan, pack_budget, pack_plan, prefill_mode  # noqa: F401  (re-exported)
 from .._rotation import rotation_enabled
 from .._serving import Checker, MemStats, maybe_sync
+from .._step import block_table
 from .pool import KushPool
 
 
@@ -138,9 +139,7 @@ class KushSGLangBackend(AttentionBackend):
         R = req.shape[0]
         g = self._graph
         bt, sl, slots = g["block_table"][:R], g["seq_lens"][:R], g["slots"][:R]
-        torch.floor_divide(self.rtp.req_to_token[req, 0:self.max_pages * PAGE:PAGE], PAGE, out=bt)
-        sl.copy_(fb.seq_lens)
-        slots.copy_(req)
+        block_table(self.rtp.req_to_token, req.contiguous(), fb.seq_lens.contiguous(), self.max_pages, out=(bt, sl, slots))
         ops = self._ops_for(self.G)
         self.forward_metadata = _Step(True, bt, sl, slots, n_splits=ops.splits(R, self.Hk, self.max_pages))
 
@@ -162,9 +161,7 @@ class KushSGLangBackend(AttentionBackend):
             return
         lens = (fb.seq_lens_cpu if fb.seq_lens_cpu is not None else fb.seq_lens.cpu()).numpy().astype(np.int64)
         pages = max(1, -(-int(lens.max()) // PAGE))
-        bt = torch.div(self.rtp.req_to_token[req.long(), 0:pages * PAGE:PAGE], PAGE,
-                       rounding_mode="floor").to(torch.int32).contiguous()
-        step = _Step(mode.is_decode(), bt, fb.seq_lens.to(torch.int32).contiguous(), req.to(torch.int32).contiguous())
+        step = _Step(mode.is_decode(), *block_table(self.rtp.req_to_token, req.contiguous(), fb.seq_lens.contiguous(), pages))
         if step.decode:
             if len(lens) > 1 and lens.min() != lens.max():
                 order = np.argsort(-lens, kind="stable").astype(np.int32)
@@ -172,7 +169,8 @@ class KushSGLangBackend(AttentionBackend):
         else:
             slots = getattr(fb, "req_pool_indices_cpu", None)
             slots = (slots if slots is not None else req.cpu()).numpy().astype(np.int64)
-            step.extend = ExtendPlan.build(list(fb.extend_seq_lens_cpu), list(fb.extend_prefix_lens_cpu), slots, bt,
+            step.extend = ExtendPlan.build(list(fb.extend_seq_lens_cpu), list(fb.extend_prefix_lens_cpu), slots,
+                                           step.block_table,
                                            kv_heads=self.Hk, head_dim=self.D, dtype=self.dtype,
                                            packed=self.prefill_mode == "packed")
         self.forward_metadata = step
