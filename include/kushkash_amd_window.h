@@ -29,12 +29,13 @@ int kush_window_decode(int head_dim, int bits, int group, int dtype, const void*
 /* kush_attend (kushkash_amd_attend.h) of queries that are the last of their keys, under a window: query row t of a
  * sequence with T rows and N >= T keys is position N - T + t. Keys left out of the rows between the sinks and the first
  * query's window change nothing, as long as they are whole: positions count in the rows given. Splits: of the tiles that a
- * row tile sees. */
+ * row tile sees. row_tiles, for ragged rows: the sum over the sequences of ceil(rows * group / (32 * waves)), which the
+ * lengths on the host give -- as many workgroups per kv head are launched; 0: as many for every sequence as the longest needs. */
 int kush_window_attend(int head_dim, int dtype, const void* q, const void* k, const void* v, void* out, float* lse,
                        const int64_t* strides, const int32_t* cu_q, const int32_t* cu_k, int32_t n_q, int32_t n_k,
                        int64_t total_q, int32_t n_seqs, int32_t hkv, int32_t group, float scale, int32_t out_f32,
                        int32_t waves, int32_t chunk, float* part_o, float* part_ml, void* stream, int32_t window,
-                       int32_t sinks);
+                       int32_t sinks, int32_t row_tiles);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,11 @@ def window_tiles(window: int, sinks: int, rows: int, group: int) -> int:
     return -(-sinks // KEYS) + (window + (rows - 1) // group) // KEYS + 2
 
 
+def row_tiles(spans, group: int, waves: int) -> int:
+    """Row tiles of all sequences of (T, ..) query rows together."""
+    return sum(-(-s[0] * group // (32 * waves)) for s in spans)
+
+
 def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
          scratch: int = PARTIAL_BYTES, window: int = 0, sinks: int = 0) -> tuple[int, int]:
     """(waves, chunk) of a call whose sequences have (T, N, count) query rows and keys. A row tile is 32 waves
@@ -133,13 +138,15 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
 
 
 @lru_cache(512)
-def _window_plan(spans: tuple, group: int, hkv: int, D: int, total: int, scratch: int, window: int, sinks: int) -> tuple[int, int, int]:
-    """plan() under a window, and the rows that the partials of split keys take (a step's layers ask for the same)."""
+def _window_plan(spans: tuple, group: int, hkv: int, D: int, total: int, scratch: int, window: int, sinks: int) -> tuple[int, int, int, int]:
+    """plan() under a window, the rows that the partials of split keys take, and the row tiles (a step's layers ask for the
+    same)."""
     waves, chunk = plan(spans, group, hkv, D, total, True, scratch, window, sinks)
+    tasks = row_tiles(spans, group, waves)
     if not chunk:
-        return waves, 0, 0
+        return waves, 0, 0, tasks
     tiles = min(-(-max(n for _, n, _ in spans) // KEYS), window_tiles(window, sinks, 32 * waves, group))
-    return waves, chunk, -(-tiles // chunk) * total * hkv * group
+    return waves, chunk, -(-tiles // chunk) * total * hkv * group, tasks
 
 
 def _native(q, k, v, scale, cu, spans, out, scratch, window, sinks):
@@ -153,8 +160,8 @@ def _native(q, k, v, scale, cu, spans, out, scratch, window, sinks):
         shape = ((n_q, n_k, q.shape[0]),)
     else:
         n_q, total, shape = cu[2], q.shape[0], tuple((t, n, 1) for t, n in spans)
-    waves, chunk, rows = _window_plan(shape, q.shape[-2] // k.shape[-2], k.shape[-2], q.shape[-1], total, scratch, window, sinks)
-    return m.attend(q, k, v, out, cu[0], cu[1], n_q, n_k, scale, window, sinks, waves, chunk, rows,
+    waves, chunk, rows, tasks = _window_plan(shape, q.shape[-2] // k.shape[-2], k.shape[-2], q.shape[-1], total, scratch, window, sinks)
+    return m.attend(q, k, v, out, cu[0], cu[1], n_q, n_k, scale, window, sinks, waves, chunk, rows, 0 if cu[0] is None else tasks,
                     torch._C._cuda_getCurrentRawStream(q.get_device()))
 
 
@@ -190,7 +197,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scal
     rows = -(-tiles // chunk) * total * Hq if chunk else 0                     # partial rows: every split's
     part = torch.empty(rows * (D + 2), dtype=torch.float32, device=dev) if chunk else None
     name = "kush_window_attend" if window else "kush_attend"
-    limit = (window, sinks) if window else ()
+    limit = (window, sinks, row_tiles(spans, group, waves) if cu is not None else 0) if window else ()
     with torch.cuda.device(dev):
         rc = getattr(_lib.lib(), name)(
             D, 1 if q.dtype == torch.float16 else 2, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),

@@ -68,9 +68,9 @@ ATTEND_SIGNATURES = {
 WINDOW_SIGNATURES = {
     # the decode list, then k, v, k_row_stride, v_row_stride, then the decode extensions, window, sinks
     "kush_window_decode": _DECODE + [_P, _P, _I64, _I64] + _DECODE_EXT + [_I32, _I32],
-    # kush_attend's list without causal, then window, sinks
+    # kush_attend's list without causal, then window, sinks, row_tiles
     "kush_window_attend": [_I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F, _I32, _I32,
-                           _I32, _P, _P, _P, _I32, _I32],
+                           _I32, _P, _P, _P, _I32, _I32, _I32],
 }
 # include/kushkash_amd_step.h
 STEP_SIGNATURES = {

@@ -87,6 +87,7 @@ struct AttendArgs {
 // With a window: of the keys 0 .. p that the query at position p sees, the last `window` and the first `sinks` alone
 struct WindowArgs : AttendArgs {
     int window, sinks;
+    int seqs, row_tiles;     // row_tiles > 0 (ragged rows): the sequences' row tiles together, the grid's y
 };
 template <typename Args>
 constexpr bool windowed = std::is_same<Args, WindowArgs>::value;
@@ -151,6 +152,31 @@ __device__ __forceinline__ Tiles key_tiles(const Args& a, const Span& s, int til
 }
 __device__ __forceinline__ int splits_of(const AttendArgs& a, int nt) { return a.chunk ? (nt + a.chunk - 1) / a.chunk : 1; }
 
+// Row tile `task` of all sequences' (bm rows each, a sequence's last ones first) as a sequence and its tile; b -1: past the
+// end. By every wave for itself, 64 sequences at a time.
+__device__ __forceinline__ void find_row_tile(const WindowArgs& a, int task, int bm, int& b, int& tile) {
+    const int lane = threadIdx.x & (WAVE - 1);
+    b = -1;
+    for (int base = 0; base < a.seqs; base += WAVE) {
+        const int s = base + lane;
+        const int tiles = s < a.seqs ? ((a.cu_q[s + 1] - a.cu_q[s]) * a.G + bm - 1) / bm : 0;
+        int end = tiles;
+#pragma unroll
+        for (int d = 1; d < WAVE; d <<= 1) {
+            const int o = __shfl_up(end, d, WAVE);
+            if (lane >= d) end += o;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(end > task);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            b = base + l;
+            tile = __builtin_amdgcn_readlane(end, l) - 1 - task;
+            return;
+        }
+        task -= __builtin_amdgcn_readlane(end, WAVE - 1);
+    }
+}
+
 // A 16-byte-per-lane load of 1 KB straight into LDS at `lds` (kush_decode.h, issue_page: m0 and its wait state)
 __device__ __forceinline__ void dma_kb(uint32_t lds, uint32_t voff, u4 rsrc) {
 #pragma clang diagnostic push
@@ -199,7 +225,9 @@ __device__ __forceinline__ void emit4(const AttendArgs& a, int64_t at, f4 v) {
         store4(a, at, v, T{});
 }
 
-// grid (Hkv * sequences, row tiles, splits), block 64 NW. Consecutive workgroups are the kv heads (and
+// grid (Hkv * sequences, row tiles, splits), block 64 NW; ragged rows under a window: (Hkv * all row tiles, 1, splits) --
+// row tiles that a shorter sequence lacks were workgroups that end at once, but they take their turns in the dealing of
+// workgroups to shader engines, so that 16 of 504 waited for a second round beside idle CUs (98 us; 73 so). Consecutive workgroups are the kv heads (and
 // sequences) of one row tile: the dispatcher deals them to the 8 XCDs in turn, so the row tiles of one kv
 // head tend to share an XCD's L2. The longest rows (the last tile) go first.
 template <int D, typename T, int NW, typename Args>
@@ -209,8 +237,14 @@ __global__ __launch_bounds__(NW * WAVE) void attend_kernel(const Args a) {
     __shared__ __align__(16) uint8_t ring[ST * 2 * A::TILE];
     const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r32 = lane & 31, hh = lane >> 5;
-    const int h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-    const int tile = gridDim.y - 1 - blockIdx.y, G = a.G;
+    const int h = blockIdx.x % a.H, G = a.G;
+    int b = blockIdx.x / a.H, tile = gridDim.y - 1 - blockIdx.y;
+    if constexpr (windowed<Args>) {
+        if (a.row_tiles > 0) {
+            find_row_tile(a, b, A::BM, b, tile);
+            if (b < 0) return;
+        }
+    }
     const Span s = span_of(a, b);
     const int rows = s.T * G;
     if (tile * A::BM >= rows) return;
@@ -469,9 +503,13 @@ static int launch_attend(const Args& a, int64_t n_seqs, int max_q, int max_k, hi
     int64_t nt = ((int64_t)max_k + KEYS - 1) / KEYS;
     if constexpr (windowed<Args>) nt = std::min(nt, window_tiles(a.window, a.sinks, BM, a.G));
     const int64_t splits = a.chunk ? (nt + a.chunk - 1) / a.chunk : 1;
+    dim3 grid((unsigned)(n_seqs * a.H), (unsigned)tiles, (unsigned)splits);
+    if constexpr (windowed<Args>) {
+        if (a.row_tiles > 0) grid.x = (unsigned)(a.row_tiles * a.H), grid.y = 1;
+    }
     if (tiles > 65535 || splits > 65535 || n_seqs * a.H > 0x7fffffff)
         return kush_fail(-2, "kush_attend: %lld row tiles x %lld splits are too many", (long long)tiles, (long long)splits);
-    attend_kernel<D, T, NW, Args><<<dim3((unsigned)(n_seqs * a.H), (unsigned)tiles, (unsigned)splits), dim3(NW * WAVE), 0, stream>>>(a);
+    attend_kernel<D, T, NW, Args><<<grid, dim3(NW * WAVE), 0, stream>>>(a);
     if (splits > 1)
         attend_merge_kernel<D, T, Args><<<dim3((unsigned)(n_seqs * a.H), (unsigned)(((int64_t)max_q * a.G + MERGE_ROWS - 1) / MERGE_ROWS)),
                                     dim3(256), 0, stream>>>(a, BM);

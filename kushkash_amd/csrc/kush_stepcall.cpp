@@ -186,7 +186,7 @@ void aligned(const at::Tensor& t, const int64_t* st) {
 }
 
 // q, k, v (checked to be of the kernel's shapes and types), out or None, cu_q, cu_k (or None), n_q, n_k, scale, window,
-// sinks, waves, chunk, partial rows, stream: the output
+// sinks, waves, chunk, partial rows, row tiles (ragged rows), stream: the output
 PyObject* attend(PyObject* const* a) {
     const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]);
     const c10::DeviceIndex dev = checked_device(q);
@@ -224,14 +224,14 @@ PyObject* attend(PyObject* const* a) {
     float *const po = part_rows ? ptr<float>(part) : nullptr, *const ml = part_rows ? po + part_rows * D : nullptr;
     const int dtype = q.scalar_type() == at::kHalf ? 1 : 2;
     const int64_t n_q = integer(a[6], 1, MOST), n_k = integer(a[7], 1, MOST), window = integer(a[9], 1, MOST),
-                  sinks = integer(a[10], 0, MOST), waves = integer(a[11], 4, 8), chunk = integer(a[12], 0, MOST);
+                  sinks = integer(a[10], 0, MOST), waves = integer(a[11], 4, 8), chunk = integer(a[12], 0, MOST), row_tiles = integer(a[14], 0, INT32_MAX);
     const float scale = (float)number(a[8], 0.0, 1e30);
-    void* const stream = (void*)integer(a[14], 0, INT64_MAX);
+    void* const stream = (void*)integer(a[15], 0, INT64_MAX);
     const void *const pq = q.data_ptr(), *const pk = k.data_ptr(), *const pv = v.data_ptr();
     void* const pout = out.data_ptr();
     CALL("kush_window_attend",
          g_attend(D, dtype, pq, pk, pv, pout, nullptr, st, cq, ck, n_q, n_k, total, seqs, Hk, Hq / Hk, scale, 0, waves, chunk, po,
-                  ml, stream, window, sinks));
+                  ml, stream, window, sinks, row_tiles));
     return wrap(out);
 }
 
@@ -371,7 +371,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(F, N) {#F, (PyCFunction)(void (*)(void))entry<F, N>, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(decode, 25), FAST(attend, 15), FAST(block_table, 6),
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(decode, 25), FAST(attend, 16), FAST(block_table, 6),
                          FAST(step_maps, 6), FAST(sample, 8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_stepcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
