@@ -17,6 +17,8 @@ KEYS = 64                        # keys per tile
 PARTIAL_BYTES = 1 << 28          # at most this much scratch for split keys
 SLOTS = {64: 4 * CUS, 128: 2 * CUS, 256: CUS}       # 4-wave workgroups the chip holds at once, by head_dim
 TILE_US = {64: 1.26, 128: 2.14, 256: 2.88}          # a key tile's time with all of them taken
+ALONE_US = {64: 0.8, 128: 1.3, 256: 1.9}            # and with a few taken
+MERGE_US = 6.0                   # what a second launch adds at least
 _Strides = ctypes.c_int64 * 15
 # torch.jit.trace, a vmap / grad / functionalize level, and dispatch modes (read on every call)
 _tracing, _transform, _modes = (torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack,
@@ -77,8 +79,8 @@ def window_tiles(window: int, sinks: int, rows: int, group: int) -> int:
 
 
 def row_tiles(spans, group: int, waves: int) -> int:
-    """Row tiles of all sequences of (T, ..) query rows together."""
-    return sum(-(-s[0] * group // (32 * waves)) for s in spans)
+    """Row tiles of all sequences of (T, N) or (T, N, count) together."""
+    return sum(-(-s[0] * group // (32 * waves)) * (s[2] if len(s) > 2 else 1) for s in spans)
 
 
 def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
@@ -101,12 +103,23 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
                it 7 (up to 13 %), and 9 of the splits that it leaves out would have gained 2-13 %.
                Not below 24 tiles (1,000 tokens over themselves: 31 us whole, 31-34 split), and into no more parts
                than min(scratch, PARTIAL_BYTES) holds the partials of.
-    With a window a row tile's keys are those that it sees, wherever they lie."""
+    With a window a row tile's keys are those that it sees, wherever they lie. Below 24 tiles, where the row tiles leave
+               half the chip idle, they are split as well, into parts of 3 tiles and more, if the tiles saved take
+               longer than the merge's launch and bytes (24 row tiles of 10 key tiles: 27.1 us whole, 21.5 in four; 3
+               of 14: 23.9, in five 16.1; 12 of 7: 15.0, in two 17.0; 144 of 7: 22.4, 28.2)."""
     longest = max([n for _, n, _ in spans])
     if window:
         longest = min(longest, window_tiles(window, sinks, 128, group) * KEYS)
     nt = -(-longest // KEYS)
     if nt < 24:
+        if window:
+            tasks = row_tiles(spans, group, 4) * hkv
+            if 0 < 2 * tasks <= SLOTS[D]:
+                chunk = max(3, -(-nt // (SLOTS[D] // tasks)))
+                row = total_q * hkv * group * (D + 2) * 4
+                cost = MERGE_US + -(-nt // chunk) * row * 2 / 2.5e6
+                if (nt - chunk) * ALONE_US[D] > cost and -(-nt // chunk) * row <= min(scratch, PARTIAL_BYTES):
+                    return 4, chunk
         return 4, 0
     if D <= 128 and longest >= 16384:
         wide = sum(c * (-(-t * group // 256)) for t, _, c in spans) * hkv              # row tiles of 8 waves
@@ -138,31 +151,41 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
 
 
 @lru_cache(512)
-def _window_plan(spans: tuple, group: int, hkv: int, D: int, total: int, scratch: int, window: int, sinks: int) -> tuple[int, int, int, int]:
-    """plan() under a window, the rows that the partials of split keys take, and the row tiles (a step's layers ask for the
-    same)."""
-    waves, chunk = plan(spans, group, hkv, D, total, True, scratch, window, sinks)
-    tasks = row_tiles(spans, group, waves)
-    if not chunk:
-        return waves, 0, 0, tasks
-    tiles = min(-(-max(n for _, n, _ in spans) // KEYS), window_tiles(window, sinks, 32 * waves, group))
-    return waves, chunk, -(-tiles // chunk) * total * hkv * group, tasks
-
-
-def _native(q, k, v, scale, cu, spans, out, scratch, window, sinks):
-    """A windowed call in native code (csrc/kush_stepcall.cpp), or None: not taken, nothing was launched."""
-    m = _lib.native()
-    n_k = k.shape[1] if cu is None else cu[3]
-    if m is None or window >= n_k:
+def _window_plan(q_shape: tuple, k_shape: tuple, spans: tuple | None, scratch: int, window: int, sinks: int) -> tuple | None:
+    """How a windowed call of these shapes runs: (n_q, n_k, waves, chunk, partial rows, row tiles of ragged rows, sequences); None where
+    the kernel does not take them, or every query sees all. A step's layers ask for the same."""
+    D, Hq, Hk = q_shape[-1], q_shape[-2], k_shape[-2]
+    if (D not in SLOTS or k_shape[-1] != D or not Hk or Hq % Hk or 0 in q_shape or 0 in k_shape or len(k_shape) != len(q_shape)
+            or len(q_shape) != (4 if spans is None else 3)):
         return None
-    if cu is None:
-        n_q, total, cu = q.shape[1], q.shape[0] * q.shape[1], (None, None)
-        shape = ((n_q, n_k, q.shape[0]),)
+    if spans is None:
+        seqs, total = ((q_shape[1], k_shape[1], q_shape[0]),), q_shape[0] * q_shape[1]
+        if k_shape[0] != q_shape[0]:
+            return None
     else:
-        n_q, total, shape = cu[2], q.shape[0], tuple((t, n, 1) for t, n in spans)
-    waves, chunk, rows, tasks = _window_plan(shape, q.shape[-2] // k.shape[-2], k.shape[-2], q.shape[-1], total, scratch, window, sinks)
-    return m.attend(q, k, v, out, cu[0], cu[1], n_q, n_k, scale, window, sinks, waves, chunk, rows, 0 if cu[0] is None else tasks,
-                    torch._C._cuda_getCurrentRawStream(q.get_device()))
+        seqs, total = tuple((t, n, 1) for t, n in spans), q_shape[0]
+        if sum(t for t, _ in spans) != total or sum(n for _, n in spans) != k_shape[0]:
+            return None
+    n_q, n_k = max(s[0] for s in seqs), max(s[1] for s in seqs)
+    group = Hq // Hk
+    if any(s[0] < 0 or s[1] < s[0] for s in seqs) or n_q * group > 1 << 22 or n_k > 1 << 30 or window >= n_k:
+        return None
+    waves, chunk = plan(seqs, group, Hk, D, total, True, scratch, window, sinks)
+    tiles = min(-(-n_k // KEYS), window_tiles(window, sinks, 32 * waves, group))
+    rows = -(-tiles // chunk) * total * Hq if chunk else 0
+    return n_q, n_k, waves, chunk, rows, 0 if spans is None else row_tiles(seqs, group, waves), q_shape[0] if spans is None else len(spans)
+
+
+def window_native(q, k, v, scale, cu, spans, out, window, sinks, scratch: int = PARTIAL_BYTES):
+    """A windowed call in native code (csrc/kush_stepcall.cpp, which checks the tensors), or None: not taken, nothing was
+    launched."""
+    m = _lib.native()
+    if m is None or not q.is_cuda or not _plain(q, k, v) or (spans is None) != (cu is None):
+        return None
+    p = _window_plan(q.shape, k.shape, None if spans is None else tuple(spans), scratch, window, sinks)
+    if p is None:
+        return None
+    return m.attend(q, k, v, out, *(cu or (None, None)), scale, window, sinks, *p, torch._C._cuda_getCurrentRawStream(q.get_device()))
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float, lse: bool = False,
@@ -175,8 +198,6 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scal
     `window` and the first `sinks` (0: all of them)."""
     D, Hq, Hk = q.shape[-1], q.shape[-2], k.shape[-2]
     group = Hq // Hk
-    if window and not lse and (o := _native(q, k, v, scale, cu, spans, out, scratch, window, sinks)) is not None:
-        return o
     if cu is None:
         seqs, n_q, n_k, total = q.shape[0], q.shape[1], k.shape[1], q.shape[0] * q.shape[1]
         cq = ck = None

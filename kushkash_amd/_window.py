@@ -75,6 +75,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     window, sinks = check_limit(window, sinks)
     if window == 0:
         raise ValueError("window_attention needs a window")
+    if (o := _attend.window_native(q, k, v, q.shape[-1] ** -0.5 if scale is None else scale, cu, spans, out, window,
+                                   sinks)) is not None:
+        return o
     packed = spans is not None
     rank = 3 if packed else 4
     if any(x.dim() != rank for x in (q, k, v)):

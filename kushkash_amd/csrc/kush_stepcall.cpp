@@ -185,13 +185,15 @@ void aligned(const at::Tensor& t, const int64_t* st) {
     for (int i = 0; i < 3; ++i) need(st[i] >= 0 && st[i] % 8 == 0);
 }
 
-// q, k, v (checked to be of the kernel's shapes and types), out or None, cu_q, cu_k (or None), n_q, n_k, scale, window,
-// sinks, waves, chunk, partial rows, row tiles (ragged rows), stream: the output
+// q, k, v (of shapes that the plan is for), out or None, cu_q, cu_k (or None), scale, window, sinks, then the plan -- n_q,
+// n_k, waves, chunk, partial rows, row tiles of ragged rows, sequences -- and the stream: the output
 PyObject* attend(PyObject* const* a) {
     const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]);
     const c10::DeviceIndex dev = checked_device(q);
     const int64_t n = q.dim(), D = q.size(n - 1), Hq = q.size(n - 2), Hk = k.size(n - 2);
-    need(k.get_device() == dev && v.get_device() == dev && (n == 3 || n == 4) && k.dim() == n && k.sizes() == v.sizes());
+    need(k.get_device() == dev && v.get_device() == dev && (n == 3 || n == 4) && k.dim() == n && k.sizes() == v.sizes() &&
+         (q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16) && k.scalar_type() == q.scalar_type() &&
+         v.scalar_type() == q.scalar_type());
     int64_t st[15] = {};
     strides_of(q, st);
     strides_of(k, st + 3);
@@ -199,21 +201,23 @@ PyObject* attend(PyObject* const* a) {
     aligned(q, st);
     aligned(k, st + 3);
     aligned(v, st + 6);
+    for (int i : {4, 7}) need(st[i] >= D && st[i] <= (1 << 23));
     const int32_t *cq = nullptr, *ck = nullptr;
-    int64_t seqs = n == 4 ? q.size(0) : 0, total = n == 4 ? seqs * q.size(1) : q.size(0);
+    const int64_t seqs = integer(a[15], 1, INT32_MAX), total = n == 4 ? seqs * q.size(1) : q.size(0);
+    need(n == 3 || q.size(0) == seqs);
     if (n == 3) {
         const at::Tensor &x = on(a[4], dev), &y = on(a[5], dev);
         need(x.scalar_type() == at::kInt && y.scalar_type() == at::kInt && x.is_contiguous() && y.is_contiguous() &&
-             x.numel() == y.numel() && x.numel() > 1);
+             x.numel() == seqs + 1 && y.numel() == seqs + 1);
         cq = ptr<int32_t>(x);
         ck = ptr<int32_t>(y);
-        seqs = x.numel() - 1;
     }
     at::Tensor out;
     if (a[3] == Py_None) {
         out = empty(q.sizes(), q.scalar_type(), q);
     } else {
         out = tensor(a[3]);
+        need(!out.requires_grad());
         need(out.get_device() == dev && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type());
     }
     strides_of(out, st + 9);
@@ -223,10 +227,12 @@ PyObject* attend(PyObject* const* a) {
     if (part_rows) part = empty({part_rows * (D + 2)}, at::kFloat, q);
     float *const po = part_rows ? ptr<float>(part) : nullptr, *const ml = part_rows ? po + part_rows * D : nullptr;
     const int dtype = q.scalar_type() == at::kHalf ? 1 : 2;
-    const int64_t n_q = integer(a[6], 1, MOST), n_k = integer(a[7], 1, MOST), window = integer(a[9], 1, MOST),
-                  sinks = integer(a[10], 0, MOST), waves = integer(a[11], 4, 8), chunk = integer(a[12], 0, MOST), row_tiles = integer(a[14], 0, INT32_MAX);
-    const float scale = (float)number(a[8], 0.0, 1e30);
-    void* const stream = (void*)integer(a[15], 0, INT64_MAX);
+    const int64_t window = integer(a[7], 1, MOST), sinks = integer(a[8], 0, MOST), n_q = integer(a[9], 1, MOST),
+                  n_k = integer(a[10], 1, MOST), waves = integer(a[11], 4, 8), chunk = integer(a[12], 0, MOST),
+                  row_tiles = integer(a[14], 0, INT32_MAX);
+    const float scale = (float)number(a[6], 0.0, 1e30);
+    need(scale > 0.0f);
+    void* const stream = (void*)integer(a[16], 0, INT64_MAX);
     const void *const pq = q.data_ptr(), *const pk = k.data_ptr(), *const pv = v.data_ptr();
     void* const pout = out.data_ptr();
     CALL("kush_window_attend",
@@ -247,9 +253,11 @@ PyObject* block_table(PyObject* const* a) {
     need(R > 0);
     at::Tensor table, l, s;
     if (a[4] == Py_None) {
-        table = empty({R, pages}, at::kInt, map);
-        l = empty({R}, at::kInt, map);
-        s = empty({R}, at::kInt, map);
+        const at::Tensor buf = empty({R * (pages + 2)}, at::kInt, map);
+        at::AutoDispatchBelowADInplaceOrView below;          // plain views, without autograd's bookkeeping
+        table = buf.as_strided({R, pages}, {std::max<int64_t>(pages, 1), 1}, 2 * R);
+        l = buf.as_strided({R}, {1}, 0);
+        s = buf.as_strided({R}, {1}, R);
     } else {
         need(PyTuple_CheckExact(a[4]) && PyTuple_GET_SIZE(a[4]) == 3);
         table = map2(PyTuple_GET_ITEM(a[4], 0), dev);
@@ -371,7 +379,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(F, N) {#F, (PyCFunction)(void (*)(void))entry<F, N>, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(decode, 25), FAST(attend, 16), FAST(block_table, 6),
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(decode, 25), FAST(attend, 17), FAST(block_table, 6),
                          FAST(step_maps, 6), FAST(sample, 8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_stepcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -119,7 +119,7 @@ def test_infinities_in_keys_that_are_hidden_from_every_row():
 def test_replays_of_a_captured_call_with_split_keys():
     dtype, D, Hk, G, T, N = torch.bfloat16, 128, 2, 4, 64, 6000
     q, k, v = (x[None].to(DEV) for x in rows(T, N, Hk, G, D, dtype, 9))
-    assert _attend._window_plan(((T, N, 1),), G, Hk, D, T, _attend.PARTIAL_BYTES, 4000, 4)[1] > 0
+    assert _attend._window_plan(q.shape, k.shape, None, _attend.PARTIAL_BYTES, 4000, 4)[3] > 0
     kk.window_attention(q, k, v, window=4000, sinks=4)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
