@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------ sampling
-// One token per row in four launches; every sum is an integer, so no order of workgroups, lanes or atomics changes it.
+// One token per row in four launches (one for a vocabulary of up to TILE tokens); every sum is an integer, so no order of
+// workgroups, lanes or atomics changes it.
 // A weight w = exp((x - max) / T) is held as a multiple of 2^-bits in 64 bits (bits such that the vocabulary's sum fits),
 // off by 2^-bits-1: far below what a 24-bit random number resolves.
 //   1. sample_max     every workgroup a piece of a row: its largest logit and where, its smallest, NaN; the row's bins
@@ -135,8 +136,12 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 //                     number and, where top-p asks, their mass: in LDS, the classes that are not empty added to the row's
 //   3. sample_pick    the classes that the cuts of top-k and top-p fall into, from the bins; the mass of every tile's
 //                     tokens above them; the tokens inside them to the row's list (a few hundred of 150,000, as a rule)
-//   4. sample_token   the list sorted: the exact cuts, ties by index; the tile that u times the kept mass falls into,
-//                     and the token in it
+//   4. sample_token   the exact cuts, ties by index: in the list, by classes of its own and a sort of the few tokens next
+//                     to the cuts; then the token in the vocabulary's order, in the list where top-k bounds it, else in the
+//                     tile that u times the kept mass falls into
+// What it has to read is the logits, once; the passes read them three times, the later ones from the caches. One row of
+// 152,000 bf16 with top-k and top-p takes 27 us (5, 5, 6 and 13: the launches' own times and the steps of one workgroup
+// over the list), 64 fp32 rows 50 (9, 11, 17 and 14: 39 MB, 8 us at the card's copy rate).
 // A list of more than LIST tokens (thousands of equal logits next to a cut) is cut by a radix search over the row instead.
 struct SampleArgs {
     const void* logits;
@@ -153,6 +158,7 @@ struct SampleArgs {
     uint64_t *mass, *sums;
     uint32_t *count, *length;
     uint2* list;
+    int index_bits;                  // of a token's index
     int64_t row0;                    // the first row of this launch (its scratch is row 0's)
 };
 
@@ -193,7 +199,7 @@ struct SampleRow {
     double c, top_p, min_p;          // c = log2 e / T
     float most, scale;               // scale: bins per logit
     int top_k, at;                   // top_k 0: off; at: the first of the order
-    bool none, greedy, by_mass, bin_mass;        // bin_mass: top-p is cut by the bins' masses
+    bool none, greedy, by_mass, bin_mass, small_k;      // bin_mass: top-p is cut by the row's bins' masses
     int bits;
     __device__ __forceinline__ double weight(float x) const { return exp2_64(x == most ? 0.0 : ((double)x - (double)most) * c); }
     // w >= 0 in multiples of 2^-bits, at least one where w is above 0
@@ -203,8 +209,9 @@ struct SampleRow {
         return w > 0.0 ? (m ? m : 1) : 0;
     }
     // the class of a logit: as d = most - x grows, never smaller
-    __device__ __forceinline__ int bin(float x) const {
-        const float d = x == most ? 0.0f : (most - x) * scale;
+    __device__ __forceinline__ int bin(float x) const { return bin(x, scale); }
+    __device__ __forceinline__ int bin(float x, float s) const {
+        const float d = x == most ? 0.0f : (most - x) * s;
         return d < (float)(BINS - 1) ? (int)d : BINS - 1;
     }
 };
@@ -227,17 +234,26 @@ struct Chunk {
     }
 };
 
-// fn(index of the first, chunk) over this thread's chunks of a tile
-template <typename T, int THREADS, typename Fn>
-__device__ __forceinline__ void tile_chunks(const T* row, int tile, int vocab, Fn&& fn) {
-    constexpr int E = Chunk<T>::E, N = TILE / (THREADS * E);
+// A thread's chunks of a tile
+template <typename T, int THREADS>
+struct TileChunks {
+    static constexpr int E = Chunk<T>::E, N = TILE / (THREADS * E);
     static_assert(N * THREADS * E == TILE, "whole chunks");
     Chunk<T> c[N];
+    __device__ __forceinline__ static int first(int tile, int j) { return tile * TILE + (j * THREADS + (int)threadIdx.x) * E; }
+    __device__ __forceinline__ void load(const T* row, int tile, int vocab) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) c[j].load(row, tile * TILE + (j * THREADS + (int)threadIdx.x) * E, vocab);
+        for (int j = 0; j < N; ++j) c[j].load(row, first(tile, j), vocab);
+    }
+    // fn(index, value) of each
+    template <typename Fn>
+    __device__ __forceinline__ void each(int tile, Fn&& fn) const {
 #pragma unroll
-    for (int j = 0; j < N; ++j) fn(tile * TILE + (j * THREADS + (int)threadIdx.x) * E, c[j]);
-}
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) fn(first(tile, j) + e, c[j].x[e]);
+    }
+};
 
 __device__ __forceinline__ SamplePart merge_parts(SamplePart a, const SamplePart& b) {
     if (b.most > a.most || (b.most == a.most && b.at < a.at)) {
@@ -271,6 +287,15 @@ __device__ __forceinline__ SamplePart wave_part(SamplePart p) {
     r.nan = __any(p.nan);
     return r;
 }
+// a logit, the indexes ascending within a thread
+__device__ __forceinline__ void merge_logit(SamplePart& p, int i, float x) {
+    p.nan |= x != x;
+    p.least = x > -__builtin_inff() ? __builtin_fminf(p.least, x) : p.least;
+    if (x > p.most) {
+        p.most = x;
+        p.at = i;
+    }
+}
 constexpr SamplePart NO_PART{-__builtin_inff(), __builtin_inff(), 0x7fffffff, 0};
 
 template <typename T>
@@ -285,19 +310,12 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_max(const SampleArgs a) 
     }
     if (piece == 0 && tid == 0) a.length[s] = 0;
     SamplePart p = NO_PART;
-    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t)
-        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
-#pragma unroll
-            for (int e = 0; e < Chunk<T>::E; ++e) {
-                const float x = c.x[e];
-                p.nan |= x != x;
-                p.least = x > -__builtin_inff() ? __builtin_fminf(p.least, x) : p.least;
-                if (x > p.most) {
-                    p.most = x;
-                    p.at = i + e;
-                }
-            }
-        });
+    const int end = min(a.tiles, (piece + 1) * a.per);
+    for (int t = piece * a.per; t < end; ++t) {
+        TileChunks<T, PIECE_THREADS> now;
+        now.load(row, t, a.vocab);
+        now.each(t, [&](int i, float x) { merge_logit(p, i, x); });
+    }
     p = wave_part(p);
     if (tid % WAVE == 0) ws[tid / WAVE] = p;
     __syncthreads();
@@ -308,11 +326,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_max(const SampleArgs a) 
 }
 
 // A row's settings and its parts put together, by every wave for itself (the same in all lanes)
-__device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, int pieces) {
-    const int64_t r = a.row0 + s;
-    SamplePart p = NO_PART;
-    for (int i = threadIdx.x % WAVE; i < pieces; i += WAVE) p = merge_parts(p, a.parts[s * pieces + i]);
-    p = wave_part(p);
+__device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t r, const SamplePart& p) {
     const double temp = a.temperatures ? (double)a.temperatures[r] : a.temperature;
     SampleRow x;
     x.top_p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
@@ -320,7 +334,8 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, 
     const int k = a.top_ks ? a.top_ks[r] : a.top_k;
     x.top_k = k > 0 && k < a.vocab ? k : 0;
     x.by_mass = x.top_p < 1.0;
-    x.bin_mass = x.by_mass && !(x.top_k && x.top_k <= SMALL_K);
+    x.small_k = x.top_k && x.top_k <= SMALL_K;
+    x.bin_mass = x.by_mass && !x.small_k;
     x.none = p.nan || p.most == -__builtin_inff();
     x.greedy = !(temp > 0.0);
     x.most = p.most;
@@ -335,30 +350,36 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, 
     return x;
 }
 
+__device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t s, int pieces) {
+    SamplePart p = NO_PART;
+    for (int i = threadIdx.x % WAVE; i < pieces; i += WAVE) p = merge_parts(p, a.parts[s * pieces + i]);
+    return sample_row(a, a.row0 + s, wave_part(p));
+}
+
 template <typename T>
 __global__ __launch_bounds__(PIECE_THREADS) void sample_bins(const SampleArgs a) {
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
     const int64_t s = blockIdx.y, r = a.row0 + s;
-    const int piece = blockIdx.x, tid = threadIdx.x;
+    const int piece = blockIdx.x, tid = threadIdx.x, end = min(a.tiles, (piece + 1) * a.per);
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     const SampleRow x = sample_row(a, s, gridDim.x);
     if (x.none || x.greedy || (!x.top_k && !x.by_mass)) return;
-    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     for (int i = tid; i < BINS; i += PIECE_THREADS) {
         mass[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
-    for (int t = piece * a.per; t < min(a.tiles, (piece + 1) * a.per); ++t)
-        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
-#pragma unroll
-            for (int e = 0; e < Chunk<T>::E; ++e) {
-                if (i + e >= a.vocab) continue;
-                const int b = x.bin(c.x[e]);
-                atomicAdd(&count[b], 1u);
-                if (x.bin_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(c.x[e])));
-            }
+    for (int t = piece * a.per; t < end; ++t) {
+        TileChunks<T, PIECE_THREADS> now;
+        now.load(row, t, a.vocab);
+        now.each(t, [&](int i, float v) {
+            if (i >= a.vocab) return;
+            const int b = x.bin(v);
+            atomicAdd(&count[b], 1u);
+            if (x.bin_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)x.fixed(x.weight(v)));
         });
+    }
     __syncthreads();
     for (int i = tid; i < BINS; i += PIECE_THREADS)
         if (count[i]) {
@@ -400,8 +421,10 @@ __device__ __forceinline__ double mass_limit(const SampleRow& x, uint64_t total)
     return __builtin_fmax(x.top_p * (double)total, 0.5);
 }
 
+// From the number and (masses) the mass of the tokens in each class; below: without masses all classes down to k are looked at
 template <int THREADS>
-__device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64_t s) {
+__device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint32_t* count, const uint64_t* mass, bool masses,
+                                                  bool below) {
     __shared__ uint64_t part[THREADS / WAVE];
     __shared__ SampleCuts cuts;
     constexpr int N = BINS / THREADS;
@@ -410,14 +433,14 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
     uint64_t m[N], ms = 0, m_all = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        c[i] = a.count[s * BINS + tid * N + i];
-        m[i] = x.bin_mass ? a.mass[s * BINS + tid * N + i] : 0;
+        c[i] = count[tid * N + i];
+        m[i] = masses ? mass[tid * N + i] : 0;
         cs += c[i];
         ms += m[i];
     }
     if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0};
     const uint32_t c1 = block_scan<THREADS>(cs, reinterpret_cast<uint32_t*>(part), c_all);
-    const uint64_t m1 = x.bin_mass ? block_scan<THREADS>(ms, part, m_all) : 0;
+    const uint64_t m1 = masses ? block_scan<THREADS>(ms, part, m_all) : 0;
     if (x.top_k) {
         uint32_t cb = c1 - cs;
         uint64_t mb = m1 - ms;
@@ -435,9 +458,9 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
     __syncthreads();
     const SampleCuts now = cuts;
     __syncthreads();
-    if (!x.bin_mass) {
+    if (!masses) {
         if (tid == 0) {
-            cuts.lo = x.by_mass ? 0 : now.k;                    // top-p as well: the list takes all that top-k keeps
+            cuts.lo = below ? 0 : now.k;
             cuts.hi = now.k;
         }
     } else {
@@ -445,7 +468,7 @@ __device__ SampleCuts sample_cuts(const SampleArgs& a, const SampleRow& x, int64
         uint64_t mb = m1 - ms;
         const double low = mass_limit(x, x.top_k ? now.before_k : m_all);
         double high = low;
-        if (x.top_k) high = mass_limit(x, now.before_k + a.mass[s * BINS + now.k]);
+        if (x.top_k) high = mass_limit(x, now.before_k + mass[now.k]);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint64_t me = mb + m[i];
@@ -472,30 +495,30 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
     __shared__ uint32_t held, place;
     const int64_t s = blockIdx.y, r = a.row0 + s;
     const int piece = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE;
+    const int end = min(a.tiles, (piece + 1) * a.per);
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     const SampleRow x = sample_row(a, s, gridDim.x);
     if (x.none || x.greedy) return;
     SampleCuts cut{BINS, BINS, BINS, 0, 0, 0};
-    if (x.top_k || x.by_mass) cut = sample_cuts<PIECE_THREADS>(a, x, s);
-    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    if (x.top_k || x.by_mass)
+        cut = sample_cuts<PIECE_THREADS>(x, a.count + s * BINS, a.mass + s * BINS, x.bin_mass, x.small_k);
     if (tid == 0) {
         held = 0;
         sum = 0;
     }
     __syncthreads();
-    const int end = min(a.tiles, (piece + 1) * a.per);
     for (int t = piece * a.per; t < end; ++t) {
         uint64_t mine = 0;
-        tile_chunks<T, PIECE_THREADS>(row, t, a.vocab, [&](int i, const Chunk<T>& c) {
-#pragma unroll
-            for (int e = 0; e < Chunk<T>::E; ++e) {
-                const int b = x.bin(c.x[e]);
-                const bool real = i + e < a.vocab;
-                if (real && b < cut.lo) {
-                    const double w = x.weight(c.x[e]);
-                    if (w >= x.min_p || i + e == x.at) mine += x.fixed(w);
-                }
-                if (real && b >= cut.lo && (b <= cut.hi || b == cut.k))
-                    gather[atomicAdd(&held, 1u)] = uint2{(uint32_t)(i + e), order_key(c.x[e])};
+        TileChunks<T, PIECE_THREADS> now;
+        now.load(row, t, a.vocab);
+        now.each(t, [&](int i, float v) {
+            if (i >= a.vocab) return;
+            const int b = x.bin(v);
+            if (b < cut.lo) {
+                const double w = x.weight(v);
+                if (w >= x.min_p || i == x.at) mine += x.fixed(w);
+            } else if (b <= cut.hi || b == cut.k) {
+                gather[atomicAdd(&held, 1u)] = uint2{(uint32_t)i, order_key(v)};
             }
         });
         if (cut.lo > 0) {
@@ -529,16 +552,244 @@ constexpr int TOKEN_THREADS = 256, MAX_TILES = (1 << 24) / TILE;
 // The order as one number, larger first: the key, then the smaller index
 __device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
 
+// The tokens of L [n], by their orders, sorted, the largest first (bitonic; the places behind them up to the power of two
+// hold 0, below every token). Up to a distance of 64 a wave's pairs lie in 128 places of its own, and its LDS operations
+// stay in order: no barrier.
+__device__ __forceinline__ void sort_orders(uint64_t* L, int size) {
+    bool apart = true;
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (apart || j > 64) __syncthreads();
+            asm volatile("" ::: "memory");
+            apart = j > 64;
+            for (int i = threadIdx.x; i < size / 2; i += TOKEN_THREADS) {
+                const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1)), q = p | j;
+                const uint64_t u = L[p], v = L[q];
+                if ((u < v) == ((p & k) == 0)) {
+                    L[p] = v;
+                    L[q] = u;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+constexpr int BORDER = 1024;                             // tokens next to the cuts that are sorted by themselves
+
+// LDS of the kernels that draw from a list
+struct DrawSpace {
+    unsigned long long mass[BINS];
+    uint32_t count[BINS];
+    uint64_t border[BORDER];
+    uint64_t part[TOKEN_THREADS / WAVE];
+    uint64_t passed;
+    int at;
+};
+
+// top-k's and top-p's cuts within L, `m` tokens sorted (largest first) that hold all of the classes that `cut` looks at, by
+// classes of width 1 / scale; masses: cut knows the masses below its classes (else L starts at the row's first token).
+// row_mass: all of the row's, for top-p alone. add(order, w, mass) for every token that is kept (weights: where they are
+// asked for). The order of the last one that is kept.
+template <typename Add>
+__device__ __forceinline__ uint64_t cut_sorted(const SampleRow& x, const uint64_t* L, int m, const SampleCuts& cut, float scale,
+                                               bool masses, uint64_t row_mass, bool weights, DrawSpace& sp, Add&& add) {
+    const int tid = threadIdx.x;
+    const auto logit = [](uint64_t order) { return key_logit((uint32_t)(order >> 32)); };
+    // of class k, the first top_k - above_k tokens
+    int k_first = m;
+    if (x.top_k) {
+        if (tid == 0) sp.at = m;
+        __syncthreads();
+        for (int i = tid; i < m; i += TOKEN_THREADS)
+            if (x.bin(logit(L[i]), scale) == cut.k && (i == 0 || x.bin(logit(L[i - 1]), scale) != cut.k)) sp.at = i;
+        __syncthreads();
+        k_first = sp.at;
+    }
+    const int keep = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : m;
+    double limit = 0.0;
+    if (x.by_mass) {
+        uint64_t total = row_mass;
+        if (x.top_k) {                                       // what top-k keeps: below its class, and its own tokens
+            uint64_t sum = 0;
+            for (int i = (masses ? k_first : 0) + tid; i < keep; i += TOKEN_THREADS) sum += x.fixed(x.weight(logit(L[i])));
+            block_scan<TOKEN_THREADS>(sum, sp.part, total);
+            total += masses ? cut.before_k : 0;
+        }
+        limit = mass_limit(x, total);
+    }
+    uint64_t before = cut.before_lo;
+    int kept = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < keep; i0 += TOKEN_THREADS) {
+        const int i = i0 + tid;
+        double w = 0.0;
+        uint64_t mine = 0, all = 0;
+        bool in = i < keep;
+        if (in && (x.by_mass || weights)) {
+            w = x.weight(logit(L[i]));
+            mine = x.fixed(w);
+        }
+        if (x.by_mass) {
+            const uint64_t run = before + block_scan<TOKEN_THREADS>(mine, sp.part, all) - mine;
+            before += all;
+            in = in && (double)run < limit;
+        }
+        if (in) add(L[i], w, mine);
+        const int now = __syncthreads_count(in);
+        kept += now;
+        if (now < TOKEN_THREADS) break;
+    }
+    const uint64_t least = kept > 0 ? L[kept - 1] : ~0ull;
+    __syncthreads();
+    return least;
+}
+
+// The token of row r from a list [n, filled up with 0 to a power of two] that holds all that may be kept. The list's tokens are
+// put into BINS classes (`fine` of them per logit), which leave a handful to sort next to the cuts; then the running sum
+// in the vocabulary's order, 10 bits of the tokens' indexes a pass.
+__device__ __forceinline__ void draw_from_list(const SampleArgs& a, int64_t r, const SampleRow& x, uint64_t* list, int n, float fine,
+                                               DrawSpace& sp) {
+    const int tid = threadIdx.x;
+    const auto logit = [](uint64_t order) { return key_logit((uint32_t)(order >> 32)); };
+    int lo = BINS;                                           // all is kept
+    uint64_t least = ~0ull;
+    if (x.top_k || x.by_mass) {
+        for (int i = tid; i < BINS; i += TOKEN_THREADS) {
+            sp.mass[i] = 0;
+            sp.count[i] = 0;
+        }
+        if (tid == 0) sp.at = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += TOKEN_THREADS) {
+            const float v = logit(list[i]);
+            const int b = x.bin(v, fine);
+            atomicAdd(&sp.count[b], 1u);
+            if (x.by_mass) atomicAdd(&sp.mass[b], (unsigned long long)x.fixed(x.weight(v)));
+        }
+        __syncthreads();
+        SampleCuts cut = sample_cuts<TOKEN_THREADS>(x, sp.count, reinterpret_cast<uint64_t*>(sp.mass), x.by_mass, false);
+        for (int i = tid; i < n; i += TOKEN_THREADS) {
+            const int b = x.bin(logit(list[i]), fine);
+            if (b >= cut.lo && (b <= cut.hi || b == cut.k)) {
+                const int at = atomicAdd(&sp.at, 1);
+                if (at < BORDER) sp.border[at] = list[i];
+            }
+        }
+        uint64_t row_mass = 0;
+        if (x.by_mass && !x.top_k) {
+            uint64_t sum = 0;
+            for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += sp.mass[i];
+            block_scan<TOKEN_THREADS>(sum, sp.part, row_mass);
+        }
+        __syncthreads();
+        int m = sp.at;
+        __syncthreads();
+        uint64_t* L = sp.border;
+        lo = cut.lo;
+        if (m > BORDER) {                                    // (equal logits by the thousands: the list as a whole)
+            L = list;
+            m = n;
+            lo = 0;
+            cut.before_lo = 0;
+        }
+        int size = 2;
+        while (size < m) size <<= 1;
+        if (L != list)
+            for (int i = m + tid; i < size; i += TOKEN_THREADS) L[i] = 0;
+        sort_orders(L, size);
+        least = cut_sorted(x, L, m, cut, fine, x.by_mass, row_mass, false, sp, [](uint64_t, double, uint64_t) {});
+    }
+    const auto mass_of = [&](uint64_t order) -> uint64_t {
+        const float v = logit(order);
+        if (!(x.bin(v, fine) < lo || order >= least)) return 0;
+        const double w = x.weight(v);
+        return w >= x.min_p || (int)~(uint32_t)order == x.at ? x.fixed(w) : 0;
+    };
+    double want = 0.0;
+    uint64_t passed = 0;
+    uint32_t prefix = 0;
+    constexpr int BITS = 10, N = BINS / TOKEN_THREADS;
+    static_assert(BINS == 1 << BITS, "a bin for each value of the digit");
+#pragma unroll 1
+    for (int top = a.index_bits; top > 0; top -= BITS) {
+        const int shift = top > BITS ? top - BITS : 0;
+        for (int i = tid; i < BINS; i += TOKEN_THREADS) sp.mass[i] = 0;
+        if (tid == 0) sp.at = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += TOKEN_THREADS) {
+            const uint32_t at = ~(uint32_t)list[i];
+            if ((at >> top) != prefix) continue;
+            const uint64_t v = mass_of(list[i]);
+            if (v) atomicAdd(&sp.mass[(at >> shift) & ((1u << (top - shift)) - 1)], (unsigned long long)v);
+        }
+        __syncthreads();
+        uint64_t v[N], sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += v[i] = sp.mass[tid * N + i];
+        uint64_t at = passed + block_scan<TOKEN_THREADS>(sum, sp.part, all) - sum;
+        // (a random number of 1 or more: the last kept token)
+        if (top == a.index_bits)
+            want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (v[i] && (double)at <= want && (double)(at + v[i]) > want) {
+                sp.at = tid * N + i;
+                sp.passed = at;
+            }
+            at += v[i];
+        }
+        __syncthreads();
+        prefix = (prefix << (top - shift)) | (uint32_t)sp.at;
+        passed = sp.passed;
+        __syncthreads();
+    }
+    if (tid == 0) a.out[r] = prefix;
+}
+
+// grid rows: vocabularies of one tile, the row in LDS as its own list (1 - 64 rows: 6 - 22 us, four launches 18 - 35;
+// 1,024 rows 11 - 44, four launches 52 - 95)
+template <typename T>
+__global__ __launch_bounds__(TOKEN_THREADS) void sample_small(const SampleArgs a) {
+    __shared__ uint64_t list[TILE];
+    __shared__ DrawSpace sp;
+    __shared__ SamplePart ws[TOKEN_THREADS / WAVE];
+    const int64_t r = a.row0 + blockIdx.x;
+    const int tid = threadIdx.x;
+    const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+    SamplePart p = NO_PART;
+    int size = 2;
+    while (size < a.vocab) size <<= 1;
+    TileChunks<T, TOKEN_THREADS> now;
+    now.load(row, 0, a.vocab);
+    now.each(0, [&](int i, float x) {
+        merge_logit(p, i, x);
+        if (i < size) list[i] = i < a.vocab ? order_of(order_key(x), i) : 0;
+    });
+    p = wave_part(p);
+    if (tid % WAVE == 0) ws[tid / WAVE] = p;
+    __syncthreads();
+    p = ws[0];
+    for (int w = 1; w < TOKEN_THREADS / WAVE; ++w) p = merge_parts(p, ws[w]);
+    const SampleRow x = sample_row(a, r, p);
+    if (x.none || x.greedy) {
+        if (tid == 0) a.out[r] = x.none ? -1 : x.at;
+        return;
+    }
+    draw_from_list(a, r, x, list, a.vocab, x.scale, sp);
+}
+
 // grid rows. What is kept of the row: tokens of classes below `lo`, and those of order `least` or above; w >= min_p.
+// Where top-k bounds the list (small_k) the token is drawn from the list alone. Else the list is the tokens of the cuts'
+// classes: sorted, added to the tiles' sums, and the token found in its tile.
 template <typename T>
 __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a, int pieces) {
     __shared__ uint64_t list[LIST];
     __shared__ unsigned long long sums[MAX_TILES];
-    __shared__ uint64_t part[TOKEN_THREADS / WAVE];
-    __shared__ uint64_t shared_mass;
-    __shared__ int shared_at;
+    __shared__ DrawSpace sp;
+    uint64_t* const part = sp.part;
     const int64_t s = blockIdx.x, r = a.row0 + s;
     const int tid = threadIdx.x;
+    const uint32_t length = a.length[s];
     const SampleRow x = sample_row(a, s, pieces);
     if (x.none || x.greedy) {
         if (tid == 0) a.out[r] = x.none ? -1 : x.at;
@@ -547,85 +798,35 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     int lo = BINS;                                       // all is kept
     uint64_t least = ~0ull;
-    const int n = x.top_k || x.by_mass ? (int)min(a.length[s], (uint32_t)0x7fffffff) : 0;
-    for (int i = tid; i < a.tiles; i += TOKEN_THREADS) sums[i] = a.sums[s * a.tiles + i];
+    const int n = x.top_k || x.by_mass ? (int)min(length, 0x7fffffffu) : 0;
     if (x.top_k || x.by_mass) {
-        const SampleCuts cut = sample_cuts<TOKEN_THREADS>(a, x, s);
-        lo = cut.lo;
+        int size = 2;
         if (n <= LIST) {
-            // sorted, the largest first (bitonic; the places behind the list hold 0, below every token). Up to a distance of
-            // 64 a wave's pairs lie in 128 places of its own, and its LDS operations stay in order: no barrier
-            int size = 2;
             while (size < n) size <<= 1;
-            for (int i = tid; i < size; i += TOKEN_THREADS)
-                list[i] = i < n ? order_of(a.list[s * LIST + i].y, a.list[s * LIST + i].x) : 0;
-            bool apart = true;
-            for (int k = 2; k <= size; k <<= 1)
-                for (int j = k >> 1; j > 0; j >>= 1) {
-                    if (apart || j > 64) __syncthreads();
-                    asm volatile("" ::: "memory");
-                    apart = j > 64;
-                    for (int i = tid; i < size / 2; i += TOKEN_THREADS) {
-                        const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1)), q = p | j;
-                        const uint64_t u = list[p], v = list[q];
-                        if ((u < v) == ((p & k) == 0)) {
-                            list[p] = v;
-                            list[q] = u;
-                        }
-                    }
-                }
-            __syncthreads();
-            const auto token = [&](int i) { return key_logit((uint32_t)(list[i] >> 32)); };
-            // of class k, the first top_k - above_k tokens
-            int k_first = n;
-            if (x.top_k) {
-                if (tid == 0) shared_at = n;
-                __syncthreads();
-                for (int i = tid; i < n; i += TOKEN_THREADS)
-                    if (x.bin(token(i)) == cut.k && (i == 0 || x.bin(token(i - 1)) != cut.k)) shared_at = i;
-                __syncthreads();
-                k_first = shared_at;
+            for (int i = tid; i < size; i += TOKEN_THREADS) {
+                const uint2 v = i < n ? a.list[s * LIST + i] : uint2{0, 0};
+                list[i] = i < n ? order_of(v.y, v.x) : 0;
             }
-            int keep = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : n;              // the list's tokens up to top-k's cut
-            double limit = 0.0;
-            if (x.by_mass) {
-                // the mass that top-k keeps: below the list's classes, and its own tokens (bin_mass false: the list starts at
-                // the first token); without top-k all of the row's
-                uint64_t sum = 0, total;
-                if (x.top_k)
-                    for (int i = (x.bin_mass ? k_first : 0) + tid; i < keep; i += TOKEN_THREADS) sum += x.fixed(x.weight(token(i)));
-                else
-                    for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
-                block_scan<TOKEN_THREADS>(sum, part, total);
-                limit = mass_limit(x, x.top_k ? cut.before_k + total : total);
-            }
-            // the tokens that are kept: their mass to their tiles
-            uint64_t before = cut.before_lo;
-            int kept = 0;
-#pragma unroll 1
-            for (int i0 = 0; i0 < keep; i0 += TOKEN_THREADS) {
-                const int i = i0 + tid;
-                double w = 0.0;
-                uint64_t m = 0, all = 0;
-                if (i < keep) {
-                    w = x.weight(token(i));
-                    m = x.fixed(w);
-                }
-                bool mine = i < keep;
-                if (x.by_mass) {
-                    const uint64_t run = before + block_scan<TOKEN_THREADS>(m, part, all) - m;
-                    before += all;
-                    mine = mine && (double)run < limit;
-                }
-                if (mine) {
-                    const uint32_t at = ~(uint32_t)list[i];
-                    if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)m);
-                }
-                const int now = __syncthreads_count(mine);
-                kept += now;
-                if (now < TOKEN_THREADS) break;
-            }
-            least = kept > 0 ? list[kept - 1] : ~0ull;
+        }
+        const SampleCuts cut = sample_cuts<TOKEN_THREADS>(x, a.count + s * BINS, a.mass + s * BINS, x.bin_mass, x.small_k);
+        if (x.small_k && n <= LIST) {
+            draw_from_list(a, r, x, list, n, x.scale * ((float)BINS / (float)(cut.k + 1)), sp);
+            return;
+        }
+        lo = cut.lo;
+        for (int i = tid; i < a.tiles; i += TOKEN_THREADS) sums[i] = a.sums[s * a.tiles + i];
+        uint64_t row_mass = 0;
+        if (x.by_mass && !x.top_k) {
+            uint64_t sum = 0;
+            for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
+            block_scan<TOKEN_THREADS>(sum, part, row_mass);
+        }
+        if (n <= LIST) {
+            sort_orders(list, size);
+            least = cut_sorted(x, list, n, cut, x.scale, x.bin_mass, row_mass, true, sp, [&](uint64_t order, double w, uint64_t mass) {
+                const uint32_t at = ~(uint32_t)order;
+                if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)mass);
+            });
         } else {
             // the token that ends what is kept, by a radix search over the row's orders: 9 bits a pass, from the top,
             // two bins to a thread
@@ -666,25 +867,25 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
                     uint64_t cb = above + block_scan<TOKEN_THREADS>(c[0] + c[1], part, unused) - c[0] - c[1];
                     uint64_t mb = above_mass + block_scan<TOKEN_THREADS>(m[0] + m[1], part, unused) - m[0] - m[1];
                     __syncthreads();
-                    if (tid == 0) shared_at = 0;
+                    if (tid == 0) sp.at = 0;
                     __syncthreads();
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const bool here = by_mass ? (double)mb < limit && !((double)(mb + m[j]) < limit)
                                                   : cb < want && cb + c[j] >= want;
                         if (here) {
-                            shared_at = b1 - j;
-                            shared_mass = mb;
+                            sp.at = b1 - j;
+                            sp.passed = mb;
                             part[0] = cb;
                         }
                         cb += c[j];
                         mb += m[j];
                     }
                     __syncthreads();
-                    prefix = (prefix << width) | (uint64_t)shared_at;
-                    above_mass = shared_mass;
+                    prefix = (prefix << width) | (uint64_t)sp.at;
+                    above_mass = sp.passed;
                     above = part[0];
-                    kept = above_mass + mass[shared_at];
+                    kept = above_mass + mass[sp.at];
                     top = shift;
                 }
                 __syncthreads();
@@ -694,11 +895,7 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
             least = 0;
             if (x.top_k) least = search(false, 0, (uint32_t)x.top_k, 0.0, total);
             if (x.by_mass) {
-                if (!x.top_k) {
-                    uint64_t sum = 0;
-                    for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
-                    block_scan<TOKEN_THREADS>(sum, part, total);
-                }
+                if (!x.top_k) total = row_mass;
                 least = search(true, least, 0, mass_limit(x, total), total);
             }
             each([&](int i, float v) {
@@ -709,6 +906,9 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         }
     }
     __syncthreads();
+    if (!x.top_k && !x.by_mass)
+        for (int i = tid; i < a.tiles; i += TOKEN_THREADS) sums[i] = a.sums[s * a.tiles + i];
+    __syncthreads();
     // the tile that the target falls into
     uint64_t run_mass = 0, all = 0;
     {
@@ -718,20 +918,20 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     }
     // (a random number of 1 or more: the last kept token)
     const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
-    if (tid == 0) shared_at = -1;
+    if (tid == 0) sp.at = -1;
     for (int t0 = 0; t0 < a.tiles; t0 += TOKEN_THREADS) {
         uint64_t here;
         const uint64_t v = t0 + tid < a.tiles ? (uint64_t)sums[t0 + tid] : 0;
         const uint64_t end = block_scan<TOKEN_THREADS>(v, part, here) + run_mass;
         if (v && (double)(end - v) <= want && (double)end > want) {
-            shared_at = t0 + tid;
-            shared_mass = end - v;
+            sp.at = t0 + tid;
+            sp.passed = end - v;
         }
         run_mass += here;
     }
     __syncthreads();
-    const int tile = shared_at;
-    run_mass = shared_mass;
+    const int tile = sp.at;
+    run_mass = sp.passed;
     __syncthreads();
     if (tile < 0) {                                      // (not reached: the first of the order has a weight)
         if (tid == 0) a.out[r] = x.at;
@@ -740,8 +940,11 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     // each thread a run of the tile's tokens, from LDS (a run and a bit apart, so that the threads read different banks)
     constexpr int E = TILE / TOKEN_THREADS, RUN = E + 1;
     float* const logit = reinterpret_cast<float*>(list);
-    for (int i = tid; i < TILE; i += TOKEN_THREADS)
-        logit[i / E * RUN + i % E] = tile * TILE + i < a.vocab ? to_f32(row[tile * TILE + i]) : -__builtin_inff();
+    {
+        TileChunks<T, TOKEN_THREADS> c;
+        c.load(row, tile, a.vocab);
+        c.each(tile, [&](int i, float v) { logit[(i - tile * TILE) / E * RUN + (i - tile * TILE) % E] = v; });
+    }
     __syncthreads();
     const auto mass_at = [&](int e) -> uint64_t {
         const int i = tile * TILE + tid * E + e;
@@ -805,8 +1008,9 @@ extern "C" int kush_step_maps(const int32_t* new_tokens, const int32_t* history,
     return kush_check_launch("kush_step_maps");
 }
 
-// Tiles of a row to a workgroup, for about three workgroups per CU
-static int64_t tiles_each(int64_t rows, int64_t tiles) { return std::min(tiles, (rows * tiles + 767) / 768); }
+// Tiles of a row to a workgroup, for about three workgroups per CU, and 4 at most (64 rows of 152,000: 4 49.8 us, 7 60.9, 2
+// 53.6, 1 67.5; 400 rows with top-p: 4 325 us, 20 413)
+static int64_t tiles_each(int64_t rows, int64_t tiles) { return std::min<int64_t>({tiles, (rows * tiles + 767) / 768, 4}); }
 
 constexpr int64_t SAMPLE_ROWS = 1024;            // rows of one launch; more go in turn, over the same scratch
 
@@ -856,13 +1060,17 @@ extern "C" int kush_sample(int dtype, const void* logits, int64_t row_stride, in
                  top_k,        temperatures, top_ps,   min_ps,                 top_ks,
                  out,          (SamplePart*)(base + at.parts),                 (uint64_t*)(base + at.mass),
                  (uint64_t*)(base + at.sums), (uint32_t*)(base + at.count),    (uint32_t*)(base + at.length),
-                 (uint2*)(base + at.list),    0};
+                 (uint2*)(base + at.list),    std::max(1, log),                0};
     const bool cuts = top_ks || top_ps || top_k > 0 || top_p < 1.0;
     hipStream_t st = (hipStream_t)stream;
     const auto go = [&](auto in) {
         using T = decltype(in);
         for (; a.row0 < rows; a.row0 += SAMPLE_ROWS) {
             const int64_t n = std::min(SAMPLE_ROWS, rows - a.row0);
+            if (vocab <= TILE) {
+                sample_small<T><<<dim3((unsigned)n), dim3(TOKEN_THREADS), 0, st>>>(a);
+                continue;
+            }
             a.per = (int)tiles_each(n, a.tiles);
             const int pieces = (a.tiles + a.per - 1) / a.per;
             const dim3 grid((unsigned)pieces, (unsigned)n);
