@@ -182,7 +182,8 @@ def window_native(q, k, v, scale, cu, spans, out, window, sinks, scratch: int = 
     m = _lib.native()
     if m is None or not q.is_cuda or not _plain(q, k, v) or (spans is None) != (cu is None):
         return None
-    p = _window_plan(q.shape, k.shape, None if spans is None else tuple(spans), scratch, window, sinks)
+    seqs = None if spans is None else tuple((int(t), int(n)) for t, n in spans)
+    p = _window_plan(q.shape, k.shape, seqs, scratch, window, sinks)
     if p is None:
         return None
     return m.attend(q, k, v, out, *(cu or (None, None)), scale, window, sinks, *p, torch._C._cuda_getCurrentRawStream(q.get_device()))

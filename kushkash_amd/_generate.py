@@ -174,7 +174,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
     if not 0.0 <= top_p or not 0.0 <= min_p:
         raise ValueError(f"top_p and min_p must be >= 0, got {top_p} and {min_p}")
     if model.config._attn_implementation != NAME:
-        enable(model, sliding_window=window == "config")
+        enable(model, sliding_window=window == "config" or (cache is not None and any(cache.windows)))
     dev = input_ids.device
     if dev.type != "cuda":
         raise ValueError("kushkash_amd.generate runs on the GPU (input_ids on a 'cuda' device under ROCm)")

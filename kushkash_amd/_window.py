@@ -1,7 +1,7 @@
 """Attention limited to a window of the last tokens and a few first ones (sinks) that stay visible: the query at
 position p sees key j <= p when j > p - window or j < sinks. The cache's decode takes the limit as Ops.decode(window=,
 sinks=); window_attention is the same limit on rows, for prompts and chunks. Kernels: csrc/kush_decode.h and
-csrc/kush_attend.hip (include/kushkash_amd_window.h)."""
+csrc/kush_attend.h (include/kushkash_amd_window.h)."""
 from __future__ import annotations
 
 import torch
@@ -71,7 +71,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     bf16 and fp16 rows of head_dim 64, 128 and 256 on the GPU, 16-byte aligned, run on the prefill attention kernel
     (forward only); anything else (fp32, other sizes, the CPU, inputs that ask for derivatives) in fp32 products. Keys
     may be left out of the rows between the sinks and the first query's window, if whole: positions count in the rows
-    given."""
+    given. Keys that a row does not see may be infinite or NaN. Their values may not, as a weight of zero times them is NaN;
+    those at least 64 rows from what any query of the sequence sees are not read."""
     window, sinks = check_limit(window, sinks)
     if window == 0:
         raise ValueError("window_attention needs a window")

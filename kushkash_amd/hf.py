@@ -193,6 +193,9 @@ def kush_attention(module, query, key, value, attention_mask, scaling=None, drop
         raise RuntimeError("kushkash attention runs on a KushHFCache: pass past_key_values=KushHFCache(...) "
                            "and use_cache=True")
     delattr(key, _ROUTE)
+    for name, what in (("s_aux", "attention with learned sink logits"), ("softcap", "attention logit softcapping")):
+        if kwargs.get(name) is not None:
+            _refuse(what)
     kv, layer = route[0].kv, route[1]
     if scaling is not None:
         kv.scale = float(scaling)
@@ -250,6 +253,8 @@ def layer_windows(cfg) -> list[int | None]:
         return [None] * cfg.num_hidden_layers
     if any(kind not in ("full_attention", "sliding_attention") for kind in kinds) or len(kinds) != cfg.num_hidden_layers:
         _refuse(f"a model with layers of {sorted(set(kinds))}")
+    if window is None and "sliding_attention" in kinds:
+        _refuse("a sliding-window model without a sliding_window in its config")
     return [window if kind == "sliding_attention" else None for kind in kinds]
 
 
