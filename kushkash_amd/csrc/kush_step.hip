@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 //                     to the cuts; then the token in the vocabulary's order, in the list where top-k bounds it, else in the
 //                     tile that u times the kept mass falls into
 // What it has to read is the logits, once; the passes read them three times, the later ones from the caches. One row of
-// 152,000 bf16 with top-k and top-p takes 27 us (5, 5, 6 and 13: the launches' own times and the steps of one workgroup
+// 152,000 bf16 with top-k 50 and top-p takes 20 us (3, 5, 6 and 6: the launches' own times and the steps of one workgroup
 // over the list), 64 fp32 rows 50 (9, 11, 17 and 14: 39 MB, 8 us at the card's copy rate).
 // A list of more than LIST tokens (thousands of equal logits next to a cut) is cut by a radix search over the row instead.
 struct SampleArgs {
@@ -644,6 +644,57 @@ __device__ __forceinline__ uint64_t cut_sorted(const SampleRow& x, const uint64_
     return least;
 }
 
+// draw_from_list's answer for n <= WAVE (what top-k 50 leaves of a row, as a rule): a token per lane, its place in the order
+// and the mass before it, there and in the vocabulary, counted over the list, a part of it per wave (one row of
+// 152,000: this kernel 13 us by draw_from_list, 7 so; lists of 150 tokens in 256 lanes took 17 and stay there)
+__device__ __forceinline__ void draw_counted(const SampleArgs& a, int64_t r, const SampleRow& x, const uint64_t* list, int n,
+                                             DrawSpace& sp) {
+    constexpr int WAVES = TOKEN_THREADS / WAVE, PART = WAVE / WAVES;
+    static_assert(BINS >= (WAVES + 1) * WAVE, "masses and parts");
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const uint64_t mine = lane < n ? list[lane] : 0;
+    const uint32_t index = ~(uint32_t)mine;
+    const double w = lane < n ? x.weight(key_logit((uint32_t)(mine >> 32))) : 0.0;
+    uint64_t mass = x.fixed(w);
+    bool in = lane < n;
+    // the sum of term(token, its mass) over the list, the same in all waves
+    const auto count = [&](auto&& term) -> uint64_t {
+        __syncthreads();
+        if (wave == 0) sp.mass[lane] = mass;
+        __syncthreads();
+        uint64_t part = 0;
+#pragma unroll
+        for (int j = wave * PART; j < wave * PART + PART; ++j)
+            if (j < n) part += term(list[j], (uint64_t)sp.mass[j]);
+        sp.mass[(wave + 1) * WAVE + lane] = part;
+        __syncthreads();
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 1; i <= WAVES; ++i) sum += sp.mass[i * WAVE + lane];
+        return sum;
+    };
+    const auto over_lanes = [](uint64_t v) {
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, WAVE);
+        return v;
+    };
+    if (x.top_k) {
+        const uint64_t place = count([&](uint64_t o, uint64_t) -> uint64_t { return o > mine; });
+        in = in && (int)place < x.top_k;
+    }
+    if (x.by_mass) {
+        const uint64_t before = count([&](uint64_t o, uint64_t m) { return o > mine ? m : 0; });
+        const double limit = mass_limit(x, over_lanes(in ? mass : 0));
+        in = in && (double)before < limit;
+    }
+    if (!in || !(w >= x.min_p || (int)index == x.at)) mass = 0;
+    const uint64_t run = count([&](uint64_t o, uint64_t m) { return (uint32_t)o > (uint32_t)mine ? m : 0; });   // (the index's complement)
+    const uint64_t all = over_lanes(mass);
+    // (a random number of 1 or more: the last kept token)
+    const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
+    if (wave == 0 && mass && (double)run <= want && (double)(run + mass) > want) a.out[r] = index;
+}
+
 // The token of row r from a list [n, filled up with 0 to a power of two] that holds all that may be kept. The list's tokens are
 // put into BINS classes (`fine` of them per logit), which leave a handful to sort next to the cuts; then the running sum
 // in the vocabulary's order, 10 bits of the tokens' indexes a pass.
@@ -807,6 +858,11 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
                 const uint2 v = i < n ? a.list[s * LIST + i] : uint2{0, 0};
                 list[i] = i < n ? order_of(v.y, v.x) : 0;
             }
+        }
+        if (x.small_k && n <= WAVE) {
+            __syncthreads();
+            draw_counted(a, r, x, list, n, sp);
+            return;
         }
         const SampleCuts cut = sample_cuts<TOKEN_THREADS>(x, a.count + s * BINS, a.mass + s * BINS, x.bin_mass, x.small_k);
         if (x.small_k && n <= LIST) {
