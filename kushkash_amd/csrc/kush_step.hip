@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 //                     to the cuts; then the token in the vocabulary's order, in the list where top-k bounds it, else in the
 //                     tile that u times the kept mass falls into
 // What it has to read is the logits, once; the passes read them three times, the later ones from the caches. One row of
-// 152,000 bf16 with top-k 50 and top-p takes 20 us (3, 5, 6 and 6: the launches' own times and the steps of one workgroup
-// over the list), 64 fp32 rows 50 (9, 11, 17 and 14: 39 MB, 8 us at the card's copy rate).
+// 152,000 bf16 with top-k 50 and top-p takes 20 us (4, 5, 5 and 6: the launches' own times and the steps of one workgroup
+// over the list), 64 fp32 rows 47 (9, 11, 13 and 14: 39 MB, 8 us at the card's copy rate).
 // A list of more than LIST tokens (thousands of equal logits next to a cut) is cut by a radix search over the row instead.
 struct SampleArgs {
     const void* logits;
@@ -409,11 +409,11 @@ __device__ __forceinline__ X block_scan(X x, X* part, X& all) {             // i
 }
 
 // The classes that the cuts fall into: everything below lo is kept (after the other cuts), lo .. hi and k are looked at
-// token by token, all else is dropped. before_lo, before_k: mass below those classes; above_k: tokens below k.
+// token by token, all else is dropped. before_lo, before_k: mass below those classes; above_k: tokens below k, in_k: in it.
 struct SampleCuts {
     int lo, hi, k;
     uint64_t before_lo, before_k;
-    uint32_t above_k;
+    uint32_t above_k, in_k;
 };
 
 // top-p's limit for a mass of `total` (at least half a unit: the first token is kept)
@@ -438,7 +438,7 @@ __device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint
         cs += c[i];
         ms += m[i];
     }
-    if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0};
+    if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0, 0};
     const uint32_t c1 = block_scan<THREADS>(cs, reinterpret_cast<uint32_t*>(part), c_all);
     const uint64_t m1 = masses ? block_scan<THREADS>(ms, part, m_all) : 0;
     if (x.top_k) {
@@ -449,6 +449,7 @@ __device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint
             if (cb < (uint32_t)x.top_k && cb + c[i] >= (uint32_t)x.top_k) {
                 cuts.k = tid * N + i;
                 cuts.above_k = cb;
+                cuts.in_k = c[i];
                 cuts.before_k = mb;
             }
             cb += c[i];
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
     const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     const SampleRow x = sample_row(a, s, gridDim.x);
     if (x.none || x.greedy) return;
-    SampleCuts cut{BINS, BINS, BINS, 0, 0, 0};
+    SampleCuts cut{BINS, BINS, BINS, 0, 0, 0, 0};
     if (x.top_k || x.by_mass)
         cut = sample_cuts<PIECE_THREADS>(x, a.count + s * BINS, a.mass + s * BINS, x.bin_mass, x.small_k);
     if (tid == 0) {
@@ -507,6 +508,25 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
         sum = 0;
     }
     __syncthreads();
+    // the list holds all that is kept, and LDS the list: no sums, one flush (64 rows of 152,000 with top-k 50: 34 us, 37 by the
+    // loop below; 400 rows 121, 140)
+    if (x.small_k && cut.above_k + cut.in_k <= GATHER) {
+        for (int t = piece * a.per; t < end; ++t) {
+            TileChunks<T, PIECE_THREADS> now;
+            now.load(row, t, a.vocab);
+            now.each(t, [&](int i, float v) {
+                if (i < a.vocab && x.bin(v) <= cut.k) gather[atomicAdd(&held, 1u)] = uint2{(uint32_t)i, order_key(v)};
+            });
+        }
+        __syncthreads();
+        const uint32_t n = held;
+        if (n == 0) return;
+        if (tid == 0) place = atomicAdd(&a.length[s], n);
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += PIECE_THREADS)
+            if (place + i < LIST) a.list[s * LIST + place + i] = gather[i];
+        return;
+    }
     for (int t = piece * a.per; t < end; ++t) {
         uint64_t mine = 0;
         TileChunks<T, PIECE_THREADS> now;
