@@ -1,6 +1,7 @@
 // C-ABI plumbing shared by every entry point: error codes and the last error message.
 // The entry points themselves live next to their kernels (kush_write.hip, kush_decode.hip,
-// kush_rotate.hip, kush_unpack.hip) and are declared in include/kushkash_amd.h.
+// kush_rotate.hip, kush_unpack.hip, declared in include/kushkash_amd.h; kush_attend.hip, kush_window_attend.hip and
+// kush_step.hip in kushkash_amd_attend.h, _window.h and _step.h).
 #include <stdarg.h>
 #include <stdio.h>
 
