@@ -4,6 +4,8 @@ sinks=); window_attention is the same limit on rows, for prompts and chunks. Ker
 csrc/kush_attend.h (include/kushkash_amd_window.h)."""
 from __future__ import annotations
 
+from itertools import accumulate
+
 import torch
 
 from . import _attend
@@ -116,8 +118,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         dst = out if out is not None and _attend.takes_out(out) else None
         if packed:
             if cu is None:
-                cu = tuple(torch.tensor([0, *(sum(s[i] for s in spans[:j + 1]) for j in range(len(spans)))], dtype=torch.int32,
-                                        device=q.device) for i in (0, 1))
+                cu = tuple(torch.tensor([0, *accumulate(s[i] for s in spans)], dtype=torch.int32, device=q.device) for i in (0, 1))
             cu = (*cu, max(t for t, _ in spans), max(n for _, n in spans))
         o = _attend.attend(q, k, v, True, scale, cu=cu, spans=spans, out=dst, window=window, sinks=sinks)
         return o if out is None or dst is not None else out.copy_(o)
