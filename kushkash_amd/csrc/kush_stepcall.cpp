@@ -96,6 +96,15 @@ at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& li
 
 PyObject* wrap(const at::Tensor& t) { return THPVariable_Wrap(t); }
 
+// A contiguous tensor over part of buf's storage, without the dispatcher (a step's maps are eleven of them)
+at::Tensor part_of(const at::Tensor& buf, at::IntArrayRef size, int64_t offset, at::ScalarType type = at::kInt) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(),
+                                                            c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    return t;
+}
+
 #define CALL(NAME, EXPR)                  \
     do {                                  \
         int rc_;                          \
@@ -254,10 +263,9 @@ PyObject* block_table(PyObject* const* a) {
     at::Tensor table, l, s;
     if (a[4] == Py_None) {
         const at::Tensor buf = empty({R * (pages + 2)}, at::kInt, map);
-        at::AutoDispatchBelowADInplaceOrView below;          // plain views, without autograd's bookkeeping
-        table = buf.as_strided({R, pages}, {std::max<int64_t>(pages, 1), 1}, 2 * R);
-        l = buf.as_strided({R}, {1}, 0);
-        s = buf.as_strided({R}, {1}, R);
+        table = part_of(buf, {R, pages}, 2 * R);
+        l = part_of(buf, {R}, 0);
+        s = part_of(buf, {R}, R);
     } else {
         need(PyTuple_CheckExact(a[4]) && PyTuple_GET_SIZE(a[4]) == 3);
         table = map2(PyTuple_GET_ITEM(a[4], 0), dev);
@@ -301,13 +309,11 @@ PyObject* step_maps(PyObject* const* a) {
     CALL("kush_step_maps",
          g_maps(pn, ph, ps, pb, row, cols, R, z[6], z[7], jobs, pages, tails, tokens, p + at[0], p + at[1], p + at[2], p + at[3],
                 p + at[4], p + at[5], p + at[6], p + at[7], p + at[8], p + at[9], (int64_t*)(p + wide), stream));
-    at::AutoDispatchBelowADInplaceOrView below;              // plain views, without autograd's bookkeeping
     PyObject* const got = PyTuple_New(11);
     if (!got) return nullptr;
-    const at::Tensor tail = buf.view(at::kLong);
     for (int i = 0; i < 10; ++i)
-        PyTuple_SET_ITEM(got, i, wrap(i == 8 ? buf.as_strided({tails, 3}, {3, 1}, at[8]) : buf.as_strided({count[i]}, {1}, at[i])));
-    PyTuple_SET_ITEM(got, 10, wrap(tail.as_strided({tokens}, {1}, wide / 2)));
+        PyTuple_SET_ITEM(got, i, wrap(i == 8 ? part_of(buf, {tails, 3}, at[8]) : part_of(buf, {count[i]}, at[i])));
+    PyTuple_SET_ITEM(got, 10, wrap(part_of(buf, {tokens}, wide / 2, at::kLong)));
     return got;
 }
 
