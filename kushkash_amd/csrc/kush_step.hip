@@ -1022,26 +1022,20 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         c.each(tile, [&](int i, float v) { logit[(i - tile * TILE) / E * RUN + (i - tile * TILE) % E] = v; });
     }
     __syncthreads();
-    const auto mass_at = [&](int e) -> uint64_t {
+    uint64_t mass[E], mine = 0, unused;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
         const int i = tile * TILE + tid * E + e;
         const float v = logit[tid * RUN + e];
-        if (i >= a.vocab || !(x.bin(v) < lo || order_of(order_key(v), i) >= least)) return 0;
         const double w = x.weight(v);
-        return w >= x.min_p || i == x.at ? x.fixed(w) : 0;
-    };
-    uint64_t mine = 0, unused;
-#pragma unroll 1
-    for (int e = 0; e < E; ++e) mine += mass_at(e);
+        const bool in = i < a.vocab && (x.bin(v) < lo || order_of(order_key(v), i) >= least) && (w >= x.min_p || i == x.at);
+        mine += mass[e] = in ? x.fixed(w) : 0;
+    }
     uint64_t before = run_mass + block_scan<TOKEN_THREADS>(mine, part, unused) - mine;
-    if (mine && (double)before <= want && (double)(before + mine) > want) {
-#pragma unroll 1
-        for (int e = 0; e < E; ++e) {
-            before += mass_at(e);
-            if ((double)before > want) {
-                a.out[r] = tile * TILE + tid * E + e;
-                break;
-            }
-        }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (mass[e] && (double)before <= want && (double)(before + mass[e]) > want) a.out[r] = tile * TILE + tid * E + e;
+        before += mass[e];
     }
 }
 
