@@ -182,15 +182,24 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 
+// a b + c, c the same in every lane and kept in scalar registers (the compiler's own form copies it for every use)
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
 // 2^t for t <= 0: e^z, |z| <= ln 2 / 2, by its Taylor polynomial of degree 12 (2e-16 off), times a power of two
 __device__ __forceinline__ double exp2_64(double t) {
     const double n = __builtin_rint(t), z = (t - n) * 0.693147180559945309417;       // 2^f = e^z
-    double p = 0.0;
     constexpr double inv[13] = {1.0,          1.0,           1.0 / 2,        1.0 / 6,          1.0 / 24,
                                 1.0 / 120,    1.0 / 720,     1.0 / 5040,     1.0 / 40320,      1.0 / 362880,
                                 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
+    double p = inv[12];
 #pragma unroll
-    for (int i = 12; i >= 0; --i) p = __builtin_fma(p, z, inv[i]);
+    for (int i = 11; i >= 3; --i) p = fma_const(p, z, inv[i]);
+#pragma unroll
+    for (int i = 2; i >= 0; --i) p = __builtin_fma(p, z, inv[i]);
     return t < -1100.0 ? 0.0 : __builtin_ldexp(p, (int)n);
 }
 
