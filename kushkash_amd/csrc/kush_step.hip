@@ -419,9 +419,10 @@ __device__ __forceinline__ X block_scan(X x, X* part, X& all) {             // i
 
 // The classes that the cuts fall into: everything below lo is kept (after the other cuts), lo .. hi and k are looked at
 // token by token, all else is dropped. before_lo, before_k: mass below those classes; above_k: tokens below k, in_k: in it.
+// all: the row's mass
 struct SampleCuts {
     int lo, hi, k;
-    uint64_t before_lo, before_k;
+    uint64_t before_lo, before_k, all;
     uint32_t above_k, in_k;
 };
 
@@ -447,7 +448,7 @@ __device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint
         cs += c[i];
         ms += m[i];
     }
-    if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0, 0};
+    if (tid == 0) cuts = SampleCuts{BINS, BINS, BINS, 0, 0, 0, 0, 0};
     const uint32_t c1 = block_scan<THREADS>(cs, reinterpret_cast<uint32_t*>(part), c_all);
     const uint64_t m1 = masses ? block_scan<THREADS>(ms, part, m_all) : 0;
     if (x.top_k) {
@@ -468,6 +469,7 @@ __device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint
     __syncthreads();
     const SampleCuts now = cuts;
     __syncthreads();
+    if (tid == 0) cuts.all = m_all;
     if (!masses) {
         if (tid == 0) {
             cuts.lo = below ? 0 : now.k;
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_pick(const SampleArgs a)
     const T* const row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
     const SampleRow x = sample_row(a, s, gridDim.x);
     if (x.none || x.greedy) return;
-    SampleCuts cut{BINS, BINS, BINS, 0, 0, 0, 0};
+    SampleCuts cut{BINS, BINS, BINS, 0, 0, 0, 0, 0};
     if (x.top_k || x.by_mass)
         cut = sample_cuts<PIECE_THREADS>(x, a.count + s * BINS, a.mass + s * BINS, x.bin_mass, x.small_k);
     if (tid == 0) {
@@ -617,11 +619,11 @@ struct DrawSpace {
 
 // top-k's and top-p's cuts within L, `m` tokens sorted (largest first) that hold all of the classes that `cut` looks at, by
 // classes of width 1 / scale; masses: cut knows the masses below its classes (else L starts at the row's first token).
-// row_mass: all of the row's, for top-p alone. add(order, w, mass) for every token that is kept (weights: where they are
+// add(order, w, mass) for every token that is kept (weights: where they are
 // asked for). The order of the last one that is kept.
 template <typename Add>
 __device__ __forceinline__ uint64_t cut_sorted(const SampleRow& x, const uint64_t* L, int m, const SampleCuts& cut, float scale,
-                                               bool masses, uint64_t row_mass, bool weights, DrawSpace& sp, Add&& add) {
+                                               bool masses, bool weights, DrawSpace& sp, Add&& add) {
     const int tid = threadIdx.x;
     const auto logit = [](uint64_t order) { return key_logit((uint32_t)(order >> 32)); };
     // of class k, the first top_k - above_k tokens
@@ -637,7 +639,7 @@ __device__ __forceinline__ uint64_t cut_sorted(const SampleRow& x, const uint64_
     const int keep = x.top_k ? k_first + (x.top_k - (int)cut.above_k) : m;
     double limit = 0.0;
     if (x.by_mass) {
-        uint64_t total = row_mass;
+        uint64_t total = cut.all;
         if (x.top_k) {                                       // what top-k keeps: below its class, and its own tokens
             uint64_t sum = 0;
             for (int i = (masses ? k_first : 0) + tid; i < keep; i += TOKEN_THREADS) sum += x.fixed(x.weight(logit(L[i])));
@@ -755,12 +757,6 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int64_t r, c
                 if (at < BORDER) sp.border[at] = list[i];
             }
         }
-        uint64_t row_mass = 0;
-        if (x.by_mass && !x.top_k) {
-            uint64_t sum = 0;
-            for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += sp.mass[i];
-            block_scan<TOKEN_THREADS>(sum, sp.part, row_mass);
-        }
         __syncthreads();
         int m = sp.at;
         __syncthreads();
@@ -777,7 +773,7 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int64_t r, c
         if (L != list)
             for (int i = m + tid; i < size; i += TOKEN_THREADS) L[i] = 0;
         sort_orders(L, size);
-        least = cut_sorted(x, L, m, cut, fine, x.by_mass, row_mass, false, sp, [](uint64_t, double, uint64_t) {});
+        least = cut_sorted(x, L, m, cut, fine, x.by_mass, false, sp, [](uint64_t, double, uint64_t) {});
     }
     const auto mass_of = [&](uint64_t order) -> uint64_t {
         const float v = logit(order);
@@ -900,15 +896,9 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         }
         lo = cut.lo;
         for (int i = tid; i < a.tiles; i += TOKEN_THREADS) sums[i] = a.sums[s * a.tiles + i];
-        uint64_t row_mass = 0;
-        if (x.by_mass && !x.top_k) {
-            uint64_t sum = 0;
-            for (int i = tid; i < BINS; i += TOKEN_THREADS) sum += a.mass[s * BINS + i];
-            block_scan<TOKEN_THREADS>(sum, part, row_mass);
-        }
         if (n <= LIST) {
             sort_orders(list, size);
-            least = cut_sorted(x, list, n, cut, x.scale, x.bin_mass, row_mass, true, sp, [&](uint64_t order, double w, uint64_t mass) {
+            least = cut_sorted(x, list, n, cut, x.scale, x.bin_mass, true, sp, [&](uint64_t order, double w, uint64_t mass) {
                 const uint32_t at = ~(uint32_t)order;
                 if (w >= x.min_p || (int)at == x.at) atomicAdd(&sums[at / TILE], (unsigned long long)mass);
             });
@@ -980,7 +970,7 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
             least = 0;
             if (x.top_k) least = search(false, 0, (uint32_t)x.top_k, 0.0, total);
             if (x.by_mass) {
-                if (!x.top_k) total = row_mass;
+                if (!x.top_k) total = cut.all;
                 least = search(true, least, 0, mass_limit(x, total), total);
             }
             each([&](int i, float v) {
