@@ -184,3 +184,29 @@ def test_refusals():
     assert kk.sample(x[:0], u[:0]).shape == (0,)
     with torch.no_grad():
         assert torch.equal(kk.sample(x.clone().requires_grad_(), u), kk.sample(x, u))
+
+
+@pytest.mark.parametrize("k", [1, 2, 62, 63, 64, 65, 66, 255, 256, 257, 2047, 2048, 2049, 4095, 5200])
+@pytest.mark.parametrize("p, m", [(1.0, 0.0), (0.6, 0.0), (0.97, 0.003)])
+def test_lists_of_every_length(k, p, m):
+    """The list that top-k leaves changes its way at 64 tokens, at a thousand next to a cut, at 2,048 and past 5,120; logits apart,
+    equal in pairs, and flat enough that a class holds many."""
+    x = torch.cat([rand(2, 9000, seed=k), rand(2, 9000, seed=k + 1, dtype=torch.bfloat16).float(), rand(2, 9000, seed=k, scale=0.01)])
+    x[3, ::2] = x[3, 1::2]
+    check(x, uniforms(6, k), k=k, p=p, m=m)
+
+
+@pytest.mark.parametrize("V", [40, 4097])
+@pytest.mark.parametrize("setting", [dict(), dict(k=20, p=0.9), dict(p=0.9)], ids=str)
+def test_more_rows_than_one_launch_takes(V, setting):
+    check(rand(1030, V, seed=V), uniforms(1030, V), **setting)
+
+
+def test_rows_that_share_their_logits():
+    """A row expanded over the batch (stride 0), and rows of a wider array."""
+    x, u = rand(1, 5001, seed=3), uniforms(9, 4)
+    got = kk.sample(x.to(DEV).expand(9, 5001), u.to(DEV), top_k=60, top_p=0.9).tolist()
+    assert got == [reference(x[0].double().numpy(), float(v), 1.0, 60, 0.9, 0.0) for v in u]
+    wide = rand(4, 6007, seed=5)
+    got = kk.sample(wide.to(DEV)[:, 3:5004], u[:4].to(DEV), top_k=60).tolist()
+    assert got == [reference(wide[i, 3:5004].double().numpy(), float(u[i]), 1.0, 60, 1.0, 0.0) for i in range(4)]
