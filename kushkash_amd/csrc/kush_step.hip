@@ -171,7 +171,7 @@ struct SamplePart {
 
 constexpr int BINS = 1024, TILE = 4096, LIST = 8192, PIECE_THREADS = 256;
 // top_k up to here: the list takes every token down to the class of top-k's cut, so that neither the bins nor the tiles need
-// masses. With top-p, this way and with masses: 64 rows of 152,000 with top_k 400 35 us and 69, 2,100 57 and 69, 4,000 66 and 70;
+// masses. With top-p, this way and with masses: 64 rows of 152,000 with top_k 2,100 57 us and 69, 4,000 66 and 70;
 // one row, whose list one workgroup draws from, 2,100 38 and 35, 4,000 46 and 37
 constexpr int SMALL_K = 2048;
 constexpr float SPAN = 64.0f;        // logits (in units of max(1, T)) that the bins cover at most
