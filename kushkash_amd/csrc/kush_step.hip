@@ -42,9 +42,9 @@ struct MapArgs {
     int64_t* slot_map;
 };
 
-// What one request adds to each array
+// What one request adds to each array (64 bits: sums of any lengths stay sums, and behind the arrays' ends)
 struct MapCounts {
-    int tokens, keys, pages, jobs, tails;
+    int64_t tokens, keys, pages, jobs, tails;
     __device__ __forceinline__ MapCounts& operator+=(const MapCounts& o) {
         tokens += o.tokens;
         keys += o.keys;
@@ -63,10 +63,11 @@ __device__ __forceinline__ int pages_left_out(const MapArgs& a, int h) {
 
 __device__ __forceinline__ MapCounts counts_of(const MapArgs& a, int t, int h) {
     const int gap = pages_left_out(a, h);
-    return MapCounts{t, h - PAGE * gap + t, h / PAGE - gap, t > 0 ? (h + t - 1) / PAGE - h / PAGE + 1 : 0, h % PAGE != 0};
+    return MapCounts{t, (int64_t)(h - PAGE * gap) + t, h / PAGE - gap, t > 0 ? (int)(((uint32_t)h + t - 1) / PAGE) - h / PAGE + 1 : 0,
+                     h % PAGE != 0};
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, WAVE);
     return x;
@@ -89,38 +90,41 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
     for (int w = 1; w < 4; ++w) before += part[w];
     const int t = max(0, a.new_tokens[r]), h = max(0, a.history[r]);
     const MapCounts mine = counts_of(a, t, h);
-    const int full = h / PAGE, gap = full - mine.pages, kept = h - PAGE * gap;
+    const int full = h / PAGE, gap = pages_left_out(a, h), kept = h - PAGE * gap;
     const int first = a.sinks / PAGE + (a.sinks % PAGE != 0);
     const int32_t* const table = a.table + (int64_t)r * a.stride;
-    const auto block = [&](int p) { return p < a.cols ? table[p] : 0; };
+    const auto block = [&](uint32_t p) { return p < a.cols ? table[p] : 0; };
     if (tid == 0 && blockIdx.y == 0) {
-        a.q_start[r] = before.tokens;
-        a.key_start[r] = before.keys;
-        a.seq_lens[r] = h + t;
+        a.q_start[r] = (int32_t)before.tokens;
+        a.key_start[r] = (int32_t)before.keys;
+        a.seq_lens[r] = (int32_t)((uint32_t)h + t);
         if (r == a.n - 1) {
-            a.q_start[a.n] = before.tokens + mine.tokens;
-            a.key_start[a.n] = before.keys + mine.keys;
+            a.q_start[a.n] = (int32_t)(before.tokens + mine.tokens);
+            a.key_start[a.n] = (int32_t)(before.keys + mine.keys);
         }
         if (mine.tails && before.tails < a.tails) {
             a.tail_blk[before.tails] = block(full);
-            int32_t* const info = a.tail_info + 3 * (int64_t)before.tails;
-            info[0] = before.keys + PAGE * mine.pages;
+            int32_t* const info = a.tail_info + 3 * before.tails;
+            info[0] = (int32_t)(before.keys + PAGE * mine.pages);
             info[1] = h % PAGE;
             info[2] = a.slots[r];
         }
     }
+    const auto room = [](int64_t n, int64_t first, int64_t size) { return (int)max((int64_t)0, min(n, size - first)); };
+    const int jobs = room(mine.jobs, before.jobs, a.jobs), pages = room(mine.pages, before.pages, a.pages),
+              tokens = room(t, before.tokens, a.tokens), key = (int)before.keys;
     const int i0 = (int)blockIdx.y * 256 + tid, step = (int)gridDim.y * 256;
-    for (int i = i0; i < mine.jobs && before.jobs + i < a.jobs; i += step) {
+    for (int i = i0; i < jobs; i += step) {
         a.job_seq[before.jobs + i] = r;
         a.job_page[before.jobs + i] = full + i;
     }
-    for (int i = i0; i < mine.pages && before.pages + i < a.pages; i += step) {
+    for (int i = i0; i < pages; i += step) {
         a.page_blk[before.pages + i] = block(i < first ? i : i + gap);
-        a.page_dst[before.pages + i] = before.keys + PAGE * i;
+        a.page_dst[before.pages + i] = key + PAGE * i;
     }
-    for (int i = i0; i < t && before.tokens + i < a.tokens; i += step) {
-        const int at = h + i;
-        a.new_dst[before.tokens + i] = before.keys + kept + i;
+    for (int i = i0; i < tokens; i += step) {
+        const uint32_t at = (uint32_t)h + i;
+        a.new_dst[before.tokens + i] = key + kept + i;
         a.slot_map[before.tokens + i] = (int64_t)block(at / PAGE) * PAGE + at % PAGE;
     }
 }

@@ -219,3 +219,26 @@ def test_refusals():
     good = kk.block_table(tokens, req, lens, 2)
     with pytest.raises(ValueError):
         kk.block_table(tokens, req, lens, 3, out=good)
+
+
+@pytest.mark.parametrize("new, history", [([2 ** 31 - 1, 2 ** 31 - 1, 4], [2 ** 31 - 1, 2 ** 31 - 1, 40]), ([1] * 300, [2 ** 31 - 1] * 300),
+                                          ([2 ** 31 - 32] * 70, [31] * 70), ([4, 4, 4], [2 ** 31 - 1, 0, 2 ** 30])])
+@pytest.mark.parametrize("window", [0, 100])
+def test_sums_of_lengths_that_pass_32_bits_stay_inside(new, history, window):
+    """Lengths that no cache has (a buffer not yet filled): nothing before or behind the arrays is written."""
+    from kushkash_amd import _lib
+    n, jobs, pages, tails, tokens, guard = len(new), 5, 6, 3, 7, 64
+    counts = [n + 1, n + 1, n, jobs, jobs, pages, pages, tails, 3 * tails, tokens, 2 * tokens]
+    buf = torch.full((sum(counts) + guard * (len(counts) + 1) + len(counts),), -99, dtype=torch.int32, device=DEV)
+    at, spots, mine = guard, [], torch.zeros(buf.numel(), dtype=torch.bool)
+    for c in counts:
+        at += at & 1                                                      # (the int64 array 8-byte aligned)
+        spots.append(buf.data_ptr() + 4 * at)
+        mine[at:at + c] = True
+        at += c + guard
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    lens, table = (i32(new), i32(history), i32(list(range(n)))), torch.ones(n, 4, dtype=torch.int32, device=DEV)
+    _lib.call("kush_step_maps", *(x.data_ptr() for x in lens), table.data_ptr(), 4, 4, n, window, 0, jobs, pages, tails, tokens, *spots,
+              torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((buf.cpu()[~mine] == -99).all())
