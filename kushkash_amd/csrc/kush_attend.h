@@ -20,7 +20,9 @@
 //   - Two waves per SIMD (8 waves at D <= 128): one's exponentials run under the other's MFMAs.
 // Measured (bf16, causal, device events): 2,048 tokens x 32 heads over 34,816 keys x 8 kv heads, D 128: 1,048 us,
 // 1,082 TFLOP/s (1,081 us, 1,049 TFLOP/s on another card), where a large bf16 matrix product reaches 1,369 and torch's
-// flash kernel 468.
+// flash kernel 468. Under a window (WindowArgs) the same kernel walks the key tiles that a row tile sees: 8,192 tokens, 2,048
+// seen, 32 x 8 heads, D 128: 284 us, 850 TFLOP/s of the pairs seen, bound as without; nine turns of up to 400 tokens over up to
+// 8,000 keys, 1,500 + 40 seen: 71 us.
 #pragma once
 
 #include <algorithm>
@@ -87,7 +89,7 @@ struct AttendArgs {
 // With a window: of the keys 0 .. p that the query at position p sees, the last `window` and the first `sinks` alone
 struct WindowArgs : AttendArgs {
     int window, sinks;
-    int seqs, row_tiles;     // row_tiles > 0 (ragged rows): the sequences' row tiles together, the grid's y
+    int seqs, row_tiles;     // row_tiles > 0 (ragged rows): the sequences' row tiles together
 };
 template <typename Args>
 constexpr bool windowed = std::is_same<Args, WindowArgs>::value;
@@ -227,9 +229,11 @@ __device__ __forceinline__ void emit4(const AttendArgs& a, int64_t at, f4 v) {
 
 // grid (Hkv * sequences, row tiles, splits), block 64 NW; ragged rows under a window: (Hkv * all row tiles, 1, splits) --
 // row tiles that a shorter sequence lacks were workgroups that end at once, but they take their turns in the dealing of
-// workgroups to shader engines, so that 16 of 504 waited for a second round beside idle CUs (98 us; 73 so). Consecutive workgroups are the kv heads (and
-// sequences) of one row tile: the dispatcher deals them to the 8 XCDs in turn, so the row tiles of one kv
-// head tend to share an XCD's L2. The longest rows (the last tile) go first.
+// workgroups to shader engines, so that 16 of 504 waited for a second round beside idle CUs (98 us; 73 so). Consecutive
+// workgroups are the kv heads (and sequences) of one row tile: the dispatcher deals them to the 8 XCDs in turn, so the row
+// tiles of one kv head tend to share an XCD's L2. The longest rows (the last tile) go first; 8,192 tokens under a window of
+// 2,048, whose last round is the first window's shorter tiles: 297 us, 303 with those dealt long and short in turn, 315
+// shortest first.
 template <int D, typename T, int NW, typename Args>
 __global__ __launch_bounds__(NW * WAVE) void attend_kernel(const Args a) {
     using A = AttendTile<D, NW>;

@@ -1,5 +1,11 @@
 // Instantiations of the decode kernel with a window for one input dtype and one rot flag, chosen by the build
 // (-DKUSH_INST_IN=float | _Float16 | kush::bf16_t, -DKUSH_INST_ROT=0 | 1): 2 and 4 waves, one or two page streams.
+//
+// o = sum of p_j v_j, p the softmax of scale q.k_j over the j < n with j >= n - window or j < sinks: the plain decode over the
+// list of pages that hold such a j, hidden tokens of those pages masked. It reads what is seen and is bound as the plain
+// decode is, by HBM, or by one launch's chain where there is little: 64 sequences of 20,000 - 32,768 tokens, 4,096 + 4 seen, int4,
+// D 128, 28 q over 4 kv heads: the kernel 32 us, 4.9 TB/s of 157 MB (37 us a launch among others, a plain decode of as many
+// tokens 34); 97 of up to 5,000, 1,111 seen, int8, D 64, 12 kv heads: 37 us; one sequence, 512 + 4 seen: 10.6 us.
 #include "kush_decode.h"
 
 #if !defined(KUSH_INST_IN) || !defined(KUSH_INST_ROT)
