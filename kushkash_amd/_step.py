@@ -232,8 +232,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         top_p < 1    of those, the tokens that have less than top_p of their mass before them;
         min_p > 0    of those, the tokens with w >= min_p;
     the first token always. The token is the first index whose running sum of kept weights, in the vocabulary's order,
-    exceeds the random number times the sum of all: the same for the same inputs, on every call. temperature 0 takes
-    the first of the order. A row with a NaN, or without a logit above -inf, gives -1. Each setting is a number, or a tensor
+    exceeds the random number times the sum of all (1 and more: the last kept one; NaN and less than 0 count as 0): the same for
+    the same inputs, on every call. temperature 0 takes the first of the order. A row with a NaN, or without a logit above -inf, gives -1. Each setting is a number, or a tensor
     with one per row (fp32; top_k int32). On the GPU."""
     if logits.is_cuda and (got := _native("sample", logits, uniforms, temperature, top_k, top_p, min_p, out)) is not None:
         return got

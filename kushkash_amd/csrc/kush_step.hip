@@ -436,6 +436,13 @@ __device__ __forceinline__ double mass_limit(const SampleRow& x, uint64_t total)
     return __builtin_fmax(x.top_p * (double)total, 0.5);
 }
 
+// What random number u leaves before its token of a kept mass of `all` (at least 1): the token's own mass passes it. 1 and more
+// leave all but the last unit, so the last kept token; NaN counts as 0. In integers: from 2^53 on a double of all - 1 is all.
+__device__ __forceinline__ uint64_t mass_before(float u, uint64_t all) {
+    const double part = (double)__builtin_fmaxf(u, 0.0f) * (double)all;
+    return u >= 1.0f ? all - 1 : min((uint64_t)part, all - 1);
+}
+
 // From the number and (masses) the mass of the tokens in each class; below: without masses all classes down to k are looked at
 template <int THREADS>
 __device__ __forceinline__ SampleCuts sample_cuts(const SampleRow& x, const uint32_t* count, const uint64_t* mass, bool masses,
@@ -726,9 +733,8 @@ __device__ __forceinline__ void draw_counted(const SampleArgs& a, int64_t r, con
     if (!in || !(w >= x.min_p || (int)index == x.at)) mass = 0;
     const uint64_t run = count([&](uint64_t o, uint64_t m) { return (uint32_t)o > (uint32_t)mine ? m : 0; });   // (the index's complement)
     const uint64_t all = over_lanes(mass);
-    // (a random number of 1 or more: the last kept token)
-    const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
-    if (wave == 0 && mass && (double)run <= want && (double)(run + mass) > want) a.out[r] = index;
+    const uint64_t want = mass_before(a.uniforms[r], all);
+    if (wave == 0 && mass && run <= want && run + mass > want) a.out[r] = index;
 }
 
 // The token of row r from a list [n, filled up with 0 to a power of two] that holds all that may be kept. The list's tokens are
@@ -786,8 +792,7 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int64_t r, c
         const double w = x.weight(v);
         return w >= x.min_p || (int)~(uint32_t)order == x.at ? x.fixed(w) : 0;
     };
-    double want = 0.0;
-    uint64_t passed = 0;
+    uint64_t want = 0, passed = 0;
     uint32_t prefix = 0;
     constexpr int BITS = 10, N = BINS / TOKEN_THREADS;
     static_assert(BINS == 1 << BITS, "a bin for each value of the digit");
@@ -808,12 +813,10 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int64_t r, c
 #pragma unroll
         for (int i = 0; i < N; ++i) sum += v[i] = sp.mass[tid * N + i];
         uint64_t at = passed + block_scan<TOKEN_THREADS>(sum, sp.part, all) - sum;
-        // (a random number of 1 or more: the last kept token)
-        if (top == a.index_bits)
-            want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
+        if (top == a.index_bits) want = mass_before(a.uniforms[r], all);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (v[i] && (double)at <= want && (double)(at + v[i]) > want) {
+            if (v[i] && at <= want && at + v[i] > want) {
                 sp.at = tid * N + i;
                 sp.passed = at;
             }
@@ -996,14 +999,13 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
         for (int t = tid; t < a.tiles; t += TOKEN_THREADS) v += sums[t];
         block_scan<TOKEN_THREADS>(v, part, all);
     }
-    // (a random number of 1 or more: the last kept token)
-    const double want = __builtin_fmin((double)__builtin_fmaxf(a.uniforms[r], 0.0f) * (double)all, (double)(all - 1));
-    if (tid == 0) sp.at = -1;
+    const uint64_t want = mass_before(a.uniforms[r], all);
+    if (tid == 0) sp.at = 0;
     for (int t0 = 0; t0 < a.tiles; t0 += TOKEN_THREADS) {
         uint64_t here;
         const uint64_t v = t0 + tid < a.tiles ? (uint64_t)sums[t0 + tid] : 0;
         const uint64_t end = block_scan<TOKEN_THREADS>(v, part, here) + run_mass;
-        if (v && (double)(end - v) <= want && (double)end > want) {
+        if (v && end - v <= want && end > want) {
             sp.at = t0 + tid;
             sp.passed = end - v;
         }
@@ -1013,10 +1015,6 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     const int tile = sp.at;
     run_mass = sp.passed;
     __syncthreads();
-    if (tile < 0) {                                      // (not reached: the first of the order has a weight)
-        if (tid == 0) a.out[r] = x.at;
-        return;
-    }
     // each thread a run of the tile's tokens, from LDS (a run and a bit apart, so that the threads read different banks)
     constexpr int E = TILE / TOKEN_THREADS, RUN = E + 1;
     float* const logit = reinterpret_cast<float*>(list);
@@ -1038,7 +1036,7 @@ __global__ __launch_bounds__(TOKEN_THREADS) void sample_token(const SampleArgs a
     uint64_t before = run_mass + block_scan<TOKEN_THREADS>(mine, part, unused) - mine;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        if (mass[e] && (double)before <= want && (double)(before + mass[e]) > want) a.out[r] = tile * TILE + tid * E + e;
+        if (mass[e] && before <= want && before + mass[e] > want) a.out[r] = tile * TILE + tid * E + e;
         before += mass[e];
     }
 }
