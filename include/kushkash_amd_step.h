@@ -46,7 +46,7 @@ int kush_step_maps(const int32_t* new_tokens, const int32_t* history, const int3
  *   min_p > 0    of those, the tokens with w >= min_p
  * the first token always. out[r] is the first index whose running sum of kept w, in the vocabulary's order, exceeds
  * uniforms[r] times the sum of all (1 and more: the last kept one; NaN and less than 0 count as 0). temperature 0: the first of the order. A row with a NaN, or with no logit above
- * -inf: -1. The parameters are one value for all rows, or (pointer not null) one per row. scratch: kush_sample_scratch(rows,
+ * -inf: -1. w is held in multiples of 2^-min(50, 63 - log2 vocab), one at least where it is above 0. The parameters are one value for all rows, or (pointer not null) one per row. scratch: kush_sample_scratch(rows,
  * vocab) bytes, 16-byte aligned, of any contents, this call's own until it has run. */
 int64_t kush_sample_scratch(int64_t rows, int64_t vocab);
 int kush_sample(int dtype, const void* logits, int64_t row_stride, int64_t rows, int64_t vocab, const float* uniforms,

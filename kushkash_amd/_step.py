@@ -234,7 +234,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     the first token always. The token is the first index whose running sum of kept weights, in the vocabulary's order,
     exceeds the random number times the sum of all (1 and more: the last kept one; NaN and less than 0 count as 0): the same for
     the same inputs, on every call. temperature 0 takes the first of the order. A row with a NaN, or without a logit above -inf, gives -1. Each setting is a number, or a tensor
-    with one per row (fp32; top_k int32). On the GPU."""
+    with one per row (fp32; top_k int32). Weights are held in multiples of 2^-min(50, 63 - log2 V) of the largest, one at least: for
+    up to 2^19 tokens the sum of all is off by less than 2^-24 of it, at 2^24 by 2^-15. On the GPU."""
     if logits.is_cuda and (got := _native("sample", logits, uniforms, temperature, top_k, top_p, min_p, out)) is not None:
         return got
     if logits.dim() != 2 or logits.dtype not in _CODE or (logits.shape[1] > 1 and logits.stride(1) != 1):

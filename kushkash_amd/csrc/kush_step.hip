@@ -132,8 +132,9 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 // ------------------------------------------------------------------ sampling
 // One token per row in four launches (one for a vocabulary of up to TILE tokens); every sum is an integer, so no order of
 // workgroups, lanes or atomics changes it.
-// A weight w = exp((x - max) / T) is held as a multiple of 2^-bits in 64 bits (bits such that the vocabulary's sum fits),
-// off by 2^-bits-1: far below what a 24-bit random number resolves.
+// A weight w = exp((x - max) / T) is held as a multiple of 2^-bits in 64 bits, one unit at least where w > 0; bits = min(50,
+// 63 - log2 vocab), such that the vocabulary's sum fits. Together the weights are off by a unit a token at most: by 2^-25 of
+// the largest at 2^19 tokens, half the least random number of 24 bits, and by 2^-15 at 2^24 tokens.
 //   1. sample_max     every workgroup a piece of a row: its largest logit and where, its smallest, NaN; the row's bins
 //                     cleared for the next launch
 //   2. sample_bins    the tokens in BINS classes of equal width below the largest logit (class 0: next to it), their
@@ -1127,7 +1128,7 @@ extern "C" int kush_sample(int dtype, const void* logits, int64_t row_stride, in
     int log = 0;
     while ((1ll << log) < vocab) ++log;
     uint8_t* const base = (uint8_t*)scratch;
-    SampleArgs a{logits,       row_stride, (int)vocab, std::min(50, 61 - log), (int)((vocab + TILE - 1) / TILE),
+    SampleArgs a{logits,       row_stride, (int)vocab, std::min(50, 63 - log), (int)((vocab + TILE - 1) / TILE),
                  0,            uniforms,   temperature, top_p,                 min_p,
                  top_k,        temperatures, top_ps,   min_ps,                 top_ks,
                  out,          (SamplePart*)(base + at.parts),                 (uint64_t*)(base + at.mass),

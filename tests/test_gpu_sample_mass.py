@@ -1,5 +1,6 @@
-"""sample where the kept mass is large: random numbers at and past the ends of their range over flat rows. Whole numbers, equal to
-the definition in 64 bits."""
+"""sample where the kept mass is large or many tiny weights add up: random numbers at and past the ends of their range over flat
+rows, and vocabularies whose tokens of next to no weight must not weigh anything together. Whole numbers, equal to the definition in
+64 bits."""
 import pytest
 import torch
 
@@ -42,3 +43,17 @@ def test_a_random_number_that_is_none():
     x = flat(8000, 64)
     assert torch.equal(kk.sample(x.to(DEV), torch.full((6,), float("nan")).to(DEV), top_k=64),
                        kk.sample(x.to(DEV), torch.zeros(6).to(DEV), top_k=64))
+
+
+@pytest.mark.parametrize("V", [151936, 262208, 1 << 19])
+def test_tokens_of_next_to_no_weight(V):
+    """One token next to all others at e^-100 of its weight: they have 2e-38 of the mass together, so the smallest random number
+    above 0 takes the one. (A weight above 0 is held as one unit at least, 2^-44 at 2^19 tokens: 2^-25 of the mass together,
+    below the smallest random number, 2^-24.)"""
+    x = torch.full((2, V), -100.0)
+    x[0, V - 1] = x[1, V // 2] = 0.0
+    for u in (2.0 ** -24, 0.25, 1 - 2.0 ** -24):
+        want = [V - 1, V // 2]
+        for kw in (dict(), dict(top_p=0.999999), dict(top_k=V - 1)):
+            got = kk.sample(x.to(DEV), torch.full((2,), u).to(DEV), **kw).tolist()
+            assert got == want, (u, kw)
