@@ -23,14 +23,19 @@ WARMUP_STEPS = 2      # eager steps (on a side stream, as torch's capture asks) 
 EOS_LAG = 2           # the host reads a step's EOS flags this many steps after queuing it
 
 
+def _by_kernel(do_sample: bool, top_p: float, min_p: float, generator: torch.Generator | None) -> bool:
+    """Whether _pick draws by the sampling kernel, whose answer for a row without a distribution is -1."""
+    return do_sample and (generator is not None or top_p < 1.0 or min_p > 0.0)
+
+
 def _pick(logits: torch.Tensor, do_sample: bool, temperature: float, top_k: int, top_p: float = 1.0, min_p: float = 0.0,
           generator: torch.Generator | None = None) -> torch.Tensor:
     """Next token per row: argmax, or a sample from softmax(logits / temperature) restricted to the
     top_k largest logits when top_k > 0 (_generate.py:23-30). With top_p, min_p or a generator: by the sampling kernel
-    (kushkash_amd.sample) from one random number per row."""
+    (kushkash_amd.sample) from one random number per row, -1 for a row with a NaN or without a logit above -inf."""
     if not do_sample:
         return logits.argmax(-1)
-    if generator is not None or top_p < 1.0 or min_p > 0.0:
+    if _by_kernel(do_sample, top_p, min_p, generator):
         u = torch.rand(logits.shape[0], dtype=torch.float32, device=logits.device, generator=generator)
         return sample(logits, u, temperature=max(temperature, 1e-5), top_k=top_k, top_p=top_p, min_p=min_p)
     z = logits.float() / max(temperature, 1e-5)
@@ -41,34 +46,55 @@ def _pick(logits: torch.Tensor, do_sample: bool, temperature: float, top_k: int,
     return torch.multinomial(torch.softmax(z, -1), 1)[:, 0]
 
 
+def _admit(tok: torch.Tensor, done: torch.Tensor, broken: torch.Tensor) -> torch.Tensor:
+    """The tokens as ids that an embedding holds: a row without one (-1) is counted in `broken`, unless it is done, and takes
+    0 until the host has read that."""
+    broken |= (tok < 0) & ~done
+    return tok.clamp(min=0)
+
+
 class _StopSignal:
     """All-rows-done detection without a host synchronization per token. Each step's `done` flags go
     to a pinned host slot of a ring by an asynchronous copy, with an event; the host reads the slot of
     the step EOS_LAG steps back (waiting for its copy if the GPU is behind), so it queues at most
     EOS_LAG steps past the step that finished every row and the GPU never idles for the check. Rows
-    already done keep emitting EOS."""
+    already done keep emitting EOS. The rows that had no distribution to draw from go the same way
+    (admit), and end the run with an error."""
 
     def __init__(self, eos: torch.Tensor, batch: int, device: torch.device):
         self.eos = eos
-        self.done = torch.zeros(batch, dtype=torch.bool, device=device)
-        self.slots = [torch.zeros(batch, dtype=torch.bool, pin_memory=True) for _ in range(EOS_LAG + 1)]
+        self.flags = torch.zeros(2, batch, dtype=torch.bool, device=device)
+        self.done, self.broken = self.flags
+        self.slots = [torch.zeros(2, batch, dtype=torch.bool, pin_memory=True) for _ in range(EOS_LAG + 1)]
         self.events = [torch.cuda.Event() for _ in range(EOS_LAG + 1)]
+
+    def admit(self, tok: torch.Tensor) -> torch.Tensor:
+        return _admit(tok, self.done, self.broken)
+
+    @staticmethod
+    def check(broken: torch.Tensor) -> None:
+        if bool(broken.any()):
+            raise RuntimeError(f"kushkash: no token could be drawn for rows {broken.nonzero()[:, 0].tolist()}: their logits have a "
+                               "NaN, or none above -inf")
 
     def finished(self, tok: torch.Tensor, step: int) -> bool:
         """Fold the newest tokens into `done`, publish them for `step`, and say whether every row was
         done EOS_LAG steps ago."""
-        self.done |= torch.isin(tok, self.eos)
+        if self.eos.numel():
+            self.done |= torch.isin(tok, self.eos)
         i = step % len(self.slots)
-        self.slots[i].copy_(self.done, non_blocking=True)
+        self.slots[i].copy_(self.flags, non_blocking=True)
         self.events[i].record()
         if step - EOS_LAG < 1:                          # steps are counted from 1
             return False
         j = (step - EOS_LAG) % len(self.slots)
         self.events[j].synchronize()
-        return bool(self.slots[j].all())
+        done, broken = self.slots[j]
+        self.check(broken)
+        return bool(done.all())
 
     def mask(self, tok: torch.Tensor) -> torch.Tensor:
-        return torch.where(self.done, self.eos[0], tok)
+        return torch.where(self.done, self.eos[0], tok) if self.eos.numel() else tok
 
 
 class _DecodeStep:
@@ -165,7 +191,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
         stats: optional dict, filled with prefill_s, prefill_history_attn_s, decode_s, decode_tokens,
             graph, eager_step_ms, graph_step_ms.
         do_sample, temperature, top_k, top_p, min_p: sample (kushkash_amd.sample has their meaning); generator: where the
-            random numbers come from (None: torch's own of the device).
+            random numbers come from (None: torch's own of the device). With top_p, min_p or a generator, a row whose logits
+            have a NaN, or none above -inf, before it is done raises a RuntimeError, EOS_LAG + 1 steps later at most.
         window, sinks: what a query sees of the tokens up to its own (KushHFCache's options): the last `window` and the
             first `sinks`; "config" takes a sliding-window model's own windows. A cache that is given brings its own.
     """
@@ -183,7 +210,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
     cache = cache if cache is not None else KushHFCache(model.config, bits=bits, max_length=total, window=window,
                                                                sinks=sinks)
     eos_ids = [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id or [])
-    stop = _StopSignal(torch.tensor(eos_ids, dtype=torch.long, device=dev), B, dev) if eos_ids else None
+    admits = _by_kernel(do_sample, top_p, min_p, generator)
+    stop = _StopSignal(torch.tensor(eos_ids, dtype=torch.long, device=dev), B, dev) if eos_ids or admits else None
 
     def forward(ids, pos):
         return model(input_ids=ids, position_ids=pos, past_key_values=cache, use_cache=True,
@@ -197,6 +225,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
         logits = forward(ids, torch.arange(c0, c0 + ids.shape[1], device=dev).expand(B, -1))
     pick = (do_sample, temperature, top_k, top_p, min_p, generator)
     tok = _pick(logits, *pick)
+    if admits:
+        tok = stop.admit(tok)
     torch.cuda.synchronize(dev)
     t1 = time.perf_counter()
 
@@ -208,10 +238,14 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, bits: int =
         if stop is not None and stop.finished(tok, i):
             break
         tok = _pick(step(tok, T0 + i - 1), *pick)
+        if admits:
+            tok = stop.admit(tok)
         if stop is not None:
             tok = stop.mask(tok)
         out.append(tok)
     torch.cuda.synchronize(dev)
+    if admits:
+        stop.check(stop.broken)
     if stats is not None:
         hist = sum(a.elapsed_time(b) for a, b in kv.profile) / 1e3 if kv.profile else 0.0
         kv.profile = None
