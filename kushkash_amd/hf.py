@@ -27,7 +27,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import _attend
 from ._attention import self_attention_blocks
-from ._window import window_attention
+from ._window import check_limit, window_attention
 from .cache import KushCache
 
 NAME = "kushkash"
@@ -115,7 +115,12 @@ class KushHFCache(Cache):
         self.bits, self.max_length, self.rotate, self.rotate_in_kernels = bits, max_length, rotate, rotate_in_kernels
         if isinstance(window, str) and window != "config":
             raise ValueError(f"window must be a number of tokens, None or 'config', got {window!r}")
-        self.windows = layer_windows(cfg) if window == "config" else [window] * self.num_layers
+        if window == "config":
+            self.windows = layer_windows(cfg)
+            check_limit(next(filter(None, self.windows), 1), sinks)          # (windows that cannot bind: no sinks either)
+        else:
+            check_limit(window, sinks)
+            self.windows = [window] * self.num_layers
         self.sinks = sinks
         self.kv: KushCache | None = None
         super().__init__(layers=[_PagedLayer(self, i) for i in range(self.num_layers)])
