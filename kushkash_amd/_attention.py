@@ -258,8 +258,11 @@ def windowed_history_attention(ops, q: torch.Tensor, k_new: torch.Tensor, v_new:
                                tail_k: torch.Tensor, scale: float, rot: bool, window: int, sinks: int) -> torch.Tensor:
     """Attention of a chunk of T queries over a cached history and the chunk itself under a window: the history's pages
     that maps (step_maps with the window; None: no history) keep are unpacked with the chunk's rows behind them by one
-    launch, and window_attention runs over the rows, in the cache's dtype. Shapes as history_attention; returns q's dtype."""
+    launch, and window_attention runs over the rows, in the cache's dtype. Shapes as history_attention, but with a key per query
+    or more, the queries being the last of them; returns q's dtype."""
     B, Hk, T, D = k_new.shape
+    if T < q.shape[2]:
+        raise ValueError(f"a chunk under a window needs a key per query, or more: got {T} for {q.shape[2]}")
     if maps is None:
         rows = [x.transpose(1, 2) for x in (q, k_new, v_new)]
         return window_attention(*rows, window=window, sinks=sinks, scale=scale).transpose(1, 2)

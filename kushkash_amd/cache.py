@@ -292,7 +292,7 @@ class KushCache:
         window, sinks = self._limits[layer]
         if window:
             n = self._tokens[layer]
-            out = windowed_history_attention(self.ops, q, k, v, self.pool[layer], self._maps(n, q.shape[2], window=window,
+            out = windowed_history_attention(self.ops, q, k, v, self.pool[layer], self._maps(n, k.shape[2], window=window,
                                              sinks=sinks) if n else None, self.tail_k[layer], self.scale,
                                              self.rot is not None, window, sinks)
         else:

@@ -1,0 +1,39 @@
+"""Chunks under a window whose keys are not one per query."""
+import pytest
+import torch
+
+import kushkash_amd as kk
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def randn(*shape, seed, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("window, sinks", [(40, 0), (90, 33), (150, 4)])
+@pytest.mark.parametrize("rows", [33, 50])
+@pytest.mark.parametrize("batch", [1, 2])
+def test_a_chunk_of_more_keys_than_queries(window, sinks, rows, batch):
+    """The chunk's queries are the last of its keys: query t stands at history + rows - T + t."""
+    T, H, G, D, n = 33, 2, 2, 128, 203
+    c = kk.KushCache(1, H, H * G, D, batch_size=batch, bits=8, device=DEV, dtype=torch.bfloat16, rotate=False, window=window, sinks=sinks)
+    c.write(0, *(randn(batch, H, n, D, seed=i) for i in (1, 2)))
+    hk, hv = (x.double().cpu() for x in c.dequantize(0))
+    q, k, v = randn(batch, H * G, T, D, seed=3), randn(batch, H, rows, D, seed=4), randn(batch, H, rows, D, seed=5)
+    got = c.attend_chunk(0, q, k, v)
+    keys, vals = (torch.cat([h, x.double().cpu()], 2).repeat_interleave(G, 1) for h, x in ((hk, k), (hv, v)))
+    p, j = torch.arange(n + rows - T, n + rows)[:, None], torch.arange(n + rows)[None]
+    s = (q.double().cpu() @ keys.transpose(2, 3) * c.scale).masked_fill((j > p) | ((j <= p - window) & (j >= sinks)), float("-inf"))
+    want = torch.softmax(s, -1) @ vals
+    # roundings to bf16 of the history's keys (through scores of about 1) and values, the weights and the output, each at most half
+    # a step, evenly spread: 2^-8 / sqrt 3 of the norm
+    assert float((got.double().cpu() - want).norm() / want.norm()) < 4 * 2.0 ** -8 / 3 ** 0.5
+
+
+def test_a_chunk_of_fewer_keys_than_queries_is_refused():
+    c = kk.KushCache(1, 2, 4, 128, device=DEV, dtype=torch.bfloat16, window=40)
+    c.write(0, randn(1, 2, 100, 128, seed=1), randn(1, 2, 100, 128, seed=2))
+    with pytest.raises(ValueError, match="key per query"):
+        c.attend_chunk(0, randn(1, 4, 33, 128, seed=3), randn(1, 2, 20, 128, seed=4), randn(1, 2, 20, 128, seed=5))
