@@ -26,7 +26,7 @@ from functools import lru_cache
 import torch
 
 from . import _attend
-from ._window import window_attention
+from ._window import limited_attention
 from ._records import PAGE, as_records, dequant_records
 
 
@@ -255,24 +255,25 @@ def _unpacked_rows(ops, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.T
 
 
 def windowed_history_attention(ops, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: torch.Tensor, maps,
-                               tail_k: torch.Tensor, scale: float, rot: bool, window: int, sinks: int) -> torch.Tensor:
+                               tail_k: torch.Tensor, scale: float, rot: bool, window: int, sinks: int,
+                               block_bytes: int = 1 << 28) -> torch.Tensor:
     """Attention of a chunk of T queries over a cached history and the chunk itself under a window: the history's pages
     that maps (step_maps with the window; None: no history) keep are unpacked with the chunk's rows behind them by one
-    launch, and window_attention runs over the rows, in the cache's dtype. Shapes as history_attention, but with a key per query
-    or more, the queries being the last of them; returns q's dtype."""
+    launch, and limited_attention runs over the rows, in the cache's dtype. Shapes as history_attention, but with a key per query
+    or more, the queries being the last of them; block_bytes bounds the attention's own scratch. Returns q's dtype."""
     B, Hk, T, D = k_new.shape
     if T < q.shape[2]:
         raise ValueError(f"a chunk under a window needs a key per query, or more: got {T} for {q.shape[2]}")
     if maps is None:
         rows = [x.transpose(1, 2) for x in (q, k_new, v_new)]
-        return window_attention(*rows, window=window, sinks=sinks, scale=scale).transpose(1, 2)
+        return limited_attention(*rows, window, sinks, scale, block_bytes=block_bytes).transpose(1, 2)
     new = [x.to(ops.dtype).transpose(1, 2).reshape(B * T, Hk, D) for x in (k_new, v_new)]
     new = [x if x.stride(2) == 1 and x.stride(1) == D else x.contiguous() for x in new]
     kp, vp = (torch.empty(maps.sizes.keys, Hk, D, dtype=ops.dtype, device=k_new.device) for _ in range(2))
     ops.unpack(cache, maps.page_blk, maps.page_dst, maps.tail_blk, maps.tail_info.view(-1), tail_k, *new, maps.new_dst, kp, vp,
                rot)
-    out = window_attention(q.to(ops.dtype).transpose(1, 2), kp.view(B, -1, Hk, D), vp.view(B, -1, Hk, D), window=window,
-                           sinks=sinks, scale=scale)
+    out = limited_attention(q.to(ops.dtype).transpose(1, 2), kp.view(B, -1, Hk, D), vp.view(B, -1, Hk, D), window, sinks, scale,
+                            block_bytes=block_bytes)
     return out.transpose(1, 2).to(q.dtype)
 
 

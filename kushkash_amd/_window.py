@@ -78,8 +78,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     window, sinks = check_limit(window, sinks)
     if window == 0:
         raise ValueError("window_attention needs a window")
-    if (o := _attend.window_native(q, k, v, q.shape[-1] ** -0.5 if scale is None else scale, cu, spans, out, window,
-                                   sinks)) is not None:
+    return limited_attention(q, k, v, window, sinks, scale, cu, spans, out)
+
+
+def limited_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int, scale: float | None = None,
+                      cu=None, spans=None, out: torch.Tensor | None = None, block_bytes: int = 1 << 28) -> torch.Tensor:
+    """window_attention of a checked limit, its scratch (partials of split keys, or scores) within block_bytes."""
+    if (o := _attend.window_native(q, k, v, q.shape[-1] ** -0.5 if scale is None else scale, cu, spans, out, window, sinks,
+                                   block_bytes)) is not None:
         return o
     packed = spans is not None
     rank = 3 if packed else 4
@@ -120,15 +126,16 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
             if cu is None:
                 cu = tuple(torch.tensor([0, *accumulate(s[i] for s in spans)], dtype=torch.int32, device=q.device) for i in (0, 1))
             cu = (*cu, max(t for t, _ in spans), max(n for _, n in spans))
-        o = _attend.attend(q, k, v, True, scale, cu=cu, spans=spans, out=dst, window=window, sinks=sinks)
+        o = _attend.attend(q, k, v, True, scale, cu=cu, spans=spans, out=dst, scratch=block_bytes, window=window, sinks=sinks)
         return o if out is None or dst is not None else out.copy_(o)
     if not packed:
-        o = _products(q, k, v, window, sinks, scale)
+        o = _products(q, k, v, window, sinks, scale, block_bytes)
     else:
         parts, a, c = [], 0, 0
         for t, n in spans:
             if t:
-                parts.append(_products(q[None, a:a + t], k[None, c:c + n], v[None, c:c + n], window, sinks, scale)[0])
+                parts.append(_products(q[None, a:a + t], k[None, c:c + n], v[None, c:c + n], window, sinks, scale,
+                                       block_bytes)[0])
             a, c = a + t, c + n
         o = torch.cat(parts)
     return o if out is None else out.copy_(o)

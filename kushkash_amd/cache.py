@@ -283,20 +283,21 @@ class KushCache:
         before the chunk is written; q [B, Hq, T, D], k, v [B, Hkv, T, D] -> [B, Hq, T, D]
         (cache.py:185-201). The history is unpacked a block of pages at a time by the unpack kernel,
         rotated back in that kernel when the cache rotates, so the attention itself runs on the
-        unrotated q and chunk; extra memory stays within ~block_bytes at any history length. Under a window the
-        history's pages that no query of the chunk sees are not unpacked, and the extra memory is the rest and the chunk."""
+        unrotated q and chunk; extra memory stays within ~block_bytes at any history length. Under a window
+        that hides any of it, the history's pages that no query of the chunk sees are not unpacked, the rest is unpacked as
+        one, and the extra memory is that, the chunk and ~block_bytes; k and v need a row per query then, or more."""
         timing = self.profile is not None and q.is_cuda
         if timing:
             ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
             ev[0].record()
         window, sinks = self._limits[layer]
-        if window:
-            n = self._tokens[layer]
+        n = self._tokens[layer]
+        if window and window + sinks < n + k.shape[2]:              # the last query does not see all
             out = windowed_history_attention(self.ops, q, k, v, self.pool[layer], self._maps(n, k.shape[2], window=window,
                                              sinks=sinks) if n else None, self.tail_k[layer], self.scale,
-                                             self.rot is not None, window, sinks)
+                                             self.rot is not None, window, sinks, block_bytes)
         else:
-            out = unpacked_history_attention(self.ops, q, k, v, self.pool[layer], self.block_table, self._tokens[layer],
+            out = unpacked_history_attention(self.ops, q, k, v, self.pool[layer], self.block_table, n,
                                              self.tail_k[layer], self.tail_idx, self.scale, self.rot is not None,
                                              block_bytes)
         if timing:

@@ -1,4 +1,4 @@
-"""Chunks under a window whose keys are not one per query."""
+"""Chunks under a window: their memory, and chunks whose keys are not one per query."""
 import pytest
 import torch
 
@@ -10,6 +10,37 @@ DEV = "cuda:0"
 
 def randn(*shape, seed, dtype=torch.bfloat16):
     return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def extra(fn):
+    """(fn's result, bytes it allocated at most beyond what was held)"""
+    fn()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    out = fn()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - held
+
+
+@pytest.mark.parametrize("rotate", [False, True])
+def test_a_window_that_hides_nothing_keeps_the_chunk_s_memory_bound(rotate):
+    """Window and sinks that cover the history and the chunk: the same output as without, in the same memory (history of 134 MB
+    in blocks of 16 MB)."""
+    H, G, D, n, T = 4, 2, 128, 65536, 64
+    plain, wide = (kk.KushCache(1, H, H * G, D, device=DEV, dtype=torch.bfloat16, rotate=rotate, **kw)
+                   for kw in (dict(), dict(window=n + T - 4, sinks=4)))
+    for a in range(0, n, 8192):
+        k, v = randn(1, H, 8192, D, seed=a + 1), randn(1, H, 8192, D, seed=a + 2)
+        for c in (plain, wide):
+            c.write(0, k, v)
+    q, k, v = randn(1, H * G, T, D, seed=3), randn(1, H, T, D, seed=4), randn(1, H, T, D, seed=5)
+    want, least = extra(lambda: plain.attend_chunk(0, q, k, v, 1 << 24))
+    got, used = extra(lambda: wide.attend_chunk(0, q, k, v, 1 << 24))
+    assert torch.equal(got, want) and used <= least + (1 << 20), f"{used >> 20} MiB, {least >> 20} without a window"
+    bound = kk.KushCache(1, H, H * G, D, device=DEV, dtype=torch.bfloat16, rotate=rotate, window=n + T - 5, sinks=4)
+    assert bound.layer_limit(0) == (n + T - 5, 4)
 
 
 @pytest.mark.parametrize("window, sinks", [(40, 0), (90, 33), (150, 4)])
