@@ -27,7 +27,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import _attend
 from ._attention import self_attention_blocks
-from ._window import check_limit, window_attention
+from ._window import check_limit, limited_attention
 from .cache import KushCache
 
 NAME = "kushkash"
@@ -156,10 +156,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     torch's memory-efficient kernel is not allowed: on ROCm its dense and varlen forms are the same kernel
     family, and its varlen form with a bottom-right causal mask has taken an illegal-address fault on this
     device. torch's half-precision math path (batched products over transposed views) is never taken either.
-    window, sinks: what a query sees of the tokens up to its own (window_attention)."""
-    if window is not None:
-        return window_attention(*(x.transpose(1, 2) for x in (q, k, v)), window=window, sinks=sinks,
-                                scale=scale).transpose(1, 2)
+    window, sinks: what a query sees of the tokens up to its own (window_attention), its scratch within block_bytes as well."""
+    window, sinks = check_limit(window, sinks)
+    if window and not (q.shape[2] == k.shape[2] <= window + sinks):              # some query does not see all
+        return limited_attention(*(x.transpose(1, 2) for x in (q, k, v)), window, sinks, scale,
+                                 block_bytes=block_bytes).transpose(1, 2)
     rows = [x.transpose(1, 2) for x in (q, k, v)]
     if k.shape[2] == q.shape[2] and _attend.takes(*rows, scale):     # else query t sees keys 0 .. t all the same
         return _attend.attend(*rows, True, scale, scratch=block_bytes).transpose(1, 2)

@@ -1,8 +1,9 @@
-"""Chunks under a window: their memory, and chunks whose keys are not one per query."""
+"""Chunks and prompts under a window: their memory, and chunks whose keys are not one per query."""
 import pytest
 import torch
 
 import kushkash_amd as kk
+from kushkash_amd.hf import prompt_attention
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -41,6 +42,27 @@ def test_a_window_that_hides_nothing_keeps_the_chunk_s_memory_bound(rotate):
     assert torch.equal(got, want) and used <= least + (1 << 20), f"{used >> 20} MiB, {least >> 20} without a window"
     bound = kk.KushCache(1, H, H * G, D, device=DEV, dtype=torch.bfloat16, rotate=rotate, window=n + T - 5, sinks=4)
     assert bound.layer_limit(0) == (n + T - 5, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window, sinks", [(4096, 0), (3000, 4)])
+def test_a_prompt_s_scratch_keeps_within_its_bound(dtype, window, sinks):
+    """prompt_attention's block_bytes holds under a window too: scores of 8 x 4,096 x 4,096 in fp32 are 537 MB, partials of split
+    bf16 keys up to 268."""
+    H, T, D = 8, 4096, 128
+    q, k, v = (randn(1, H, T, D, seed=i, dtype=dtype) for i in range(3))
+    rows = 4 * q.numel() * (6 if dtype == torch.float32 else 1)              # the output, fp32 rows of a block's keys and values
+    out, used = extra(lambda: prompt_attention(q, k, v, D ** -0.5, 1 << 22, window=window, sinks=sinks))
+    assert used <= rows + (1 << 24), f"{used >> 20} MiB"
+    at = torch.arange(T, device=DEV)
+    hidden = (at[None] > at[:, None]) | ((at[None] <= at[:, None] - window) & (at[None] >= sinks))
+    for h in (0, 5):
+        s = (q[0, h].double() @ k[0, h].double().t().contiguous() * D ** -0.5).masked_fill_(hidden, float("-inf"))
+        want = torch.softmax(s, -1) @ v[0, h].double()
+        # bf16: the weights' rounding, half a step (2^-8) above the division and below, and the output's; fp32: a score off by
+        # 128 roundings of 2^-24 of its terms' sum, below 15, which counts twice in a weight
+        off = 3 * 2.0 ** -8 if dtype == torch.bfloat16 else 2 * 128 * 2.0 ** -24 * 15
+        assert float((out[0, h].double() - want).abs().max()) <= off * float(v.abs().max())
 
 
 @pytest.mark.parametrize("window, sinks", [(40, 0), (90, 33), (150, 4)])
