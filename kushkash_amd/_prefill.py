@@ -8,8 +8,8 @@ kushkash/vllm/backend.py:385-475, :807-880.
 Host side, once per step (``ExtendPlan``): the write jobs (one per (request, logical page) the new
 tokens touch), and the attention groups: consecutive requests whose K + V, history and new tokens
 together, fit a byte budget are packed end to end; a request over the budget alone (and every request
-in loop mode) takes its history in blocks of pages. The lengths and tail slots go to the device in one copy;
-every index array is built from them there (_step.step_maps).
+in loop mode) takes its history in blocks of pages. One copy takes the lengths and tail slots to the device, which the packed
+groups' index arrays are built from there (_step.step_maps), and the write's jobs, where no group holds the whole step.
 
 Device side, per layer (``ExtendPlan.attend``, before the step's write): per packed group one launch of
 the unpack kernel builds every request's keys [history pages | partial page (K from the tail, V from
@@ -30,7 +30,7 @@ import torch
 from ._attention import ragged_attention, unpacked_history_attention
 from ._ops import PAGE
 from ._serving import torch_unpack, unpack_mode
-from ._step import map_sizes, step_maps
+from ._step import MOST_REQUESTS, map_sizes, step_maps
 
 
 def record_bits() -> int:
@@ -133,6 +133,14 @@ def group_requests(new_tokens: np.ndarray, history: np.ndarray, bytes_per_key: i
     return out
 
 
+def write_jobs(new_tokens: np.ndarray, history: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """(request, logical page) of every page that each request's new tokens touch (pages_touched)."""
+    first = history // PAGE
+    count = np.where(new_tokens > 0, (history + new_tokens - 1) // PAGE - first + 1, 0)
+    seq = np.repeat(np.arange(len(count)), count)
+    return seq, np.arange(len(seq)) - (np.cumsum(count) - count - first)[seq]
+
+
 def _host_to_device(arr: np.ndarray, device: torch.device) -> torch.Tensor:
     return torch.from_numpy(arr).to(device)
 
@@ -152,8 +160,8 @@ class ExtendPlan:
     @classmethod
     def build(cls, new_tokens, history, slots, block_table: torch.Tensor, *, kv_heads: int, head_dim: int,
               dtype: torch.dtype, packed: bool = True, budget: int | None = None, upload=None) -> "ExtendPlan":
-        """upload(int32 numpy array) -> device tensor: how the step's one host -> device copy (its lengths and slots) is
-        made (default: a plain copy to the block table's device)."""
+        """upload(int32 numpy array) -> device tensor: how the step's one host -> device copy is made (default: a plain copy
+        to the block table's device)."""
         q = np.asarray(new_tokens, dtype=np.int64)
         h = np.asarray(history, dtype=np.int64)
         slots = np.asarray(slots, dtype=np.int64)
@@ -163,31 +171,49 @@ class ExtendPlan:
         elem = torch.empty((), dtype=dtype).element_size()
         layout = group_requests(q, h, 2 * kv_heads * head_dim * elem, pack_budget() if budget is None else budget,
                                 packed)
-        # the lengths and slots go over; every index array is built from them on the device
-        lens = np.concatenate([q, h, slots]).astype(np.int32)
-        dev = (upload or (lambda a: _host_to_device(a, block_table.device)))(lens)
-        parts = dev[:R], dev[R:2 * R], dev[2 * R:3 * R]
 
-        def maps(r0, r1, writes):
-            sizes = map_sizes(q[r0:r1].tolist(), h[r0:r1].tolist())
-            return step_maps(*(x[r0:r1] for x in parts), block_table[r0:r1], sizes.writes() if writes else sizes)
+        def by_maps(r0, r1, is_packed):
+            return is_packed and r1 - r0 <= MOST_REQUESTS
 
-        whole = maps(0, R, writes=len(layout) != 1 or not layout[0][2])
-        plan = cls(whole.q_start, whole.job_seq, whole.job_page, q_start_host=[int(x) for x in q_start],
-                   history_host=[int(x) for x in h])
+        # one copy: the lengths and slots that groups' maps are built from, the arrays of the others
+        one = len(layout) == 1 and by_maps(*layout[0])           # its maps are the whole step's
+        host, plans = [], []
+        if any(by_maps(*g) for g in layout):
+            host = [q, h, slots]
+        if not one:
+            host += [q_start, *write_jobs(q, h)]
         for r0, r1, is_packed in layout:
+            plans.append(None if not is_packed or by_maps(r0, r1, is_packed) else pack_plan(q[r0:r1], h[r0:r1], slots[r0:r1]))
+            if (p := plans[-1]) is not None:
+                host += [p.key_start, q_start[r0:r1 + 1] - q_start[r0], r0 + p.page_req, p.page_index, p.page_dst,
+                         r0 + p.tail_req, h[r0 + p.tail_req] // PAGE, p.tail_info.reshape(-1), p.new_dst]
+        dev = (upload or (lambda a: _host_to_device(a, block_table.device)))(np.concatenate(host).astype(np.int32))
+        ends = np.cumsum([len(a) for a in host])
+        views = iter([dev[int(e) - len(a):int(e)] for a, e in zip(host, ends)])
+        lens = [next(views) for _ in range(3)] if any(by_maps(*g) for g in layout) else None
+        write = None if one else [next(views) for _ in range(3)]
+        groups = []
+        for (r0, r1, is_packed), p in zip(layout, plans):
             g = Group(r0, r1, is_packed)
             if is_packed:
-                m = whole if (r0, r1) == (0, R) else maps(r0, r1, writes=False)
-                g.cu_k, g.cu_q, g.page_blk, g.page_dst = m.key_start, m.q_start, m.page_blk, m.page_dst
-                g.tail_blk, g.tail_info, g.new_dst = m.tail_blk, m.tail_info.view(-1), m.new_dst
+                if p is None:
+                    m = step_maps(*(x[r0:r1] for x in lens), block_table[r0:r1], map_sizes(q[r0:r1].tolist(), h[r0:r1].tolist()))
+                    g.cu_k, g.cu_q, g.page_blk, g.page_dst = m.key_start, m.q_start, m.page_blk, m.page_dst
+                    g.tail_blk, g.tail_info, g.new_dst = m.tail_blk, m.tail_info.view(-1), m.new_dst
+                    if one:
+                        write = m.q_start, m.job_seq, m.job_page
+                else:
+                    g.cu_k, g.cu_q, page_req, page_index, g.page_dst, tail_req, tail_page, g.tail_info, g.new_dst = (
+                        next(views) for _ in range(9))
+                    g.page_blk = block_table[page_req.long(), page_index.long()].contiguous()
+                    g.tail_blk = block_table[tail_req.long(), tail_page.long()].contiguous()
                 g.key_start = [0, *(int(x) for x in np.cumsum(total[r0:r1]))]
                 g.n_keys = g.key_start[-1]
                 g.has_history = bool(h[r0:r1].any())
                 g.max_q = int(q[r0:r1].max())
                 g.max_k = int(total[r0:r1].max())
-            plan.groups.append(g)
-        return plan
+            groups.append(g)
+        return cls(*write, groups, [int(x) for x in q_start], [int(x) for x in h])
 
     def attend(self, ops, q3: torch.Tensor, k3: torch.Tensor, v3: torch.Tensor, cache: torch.Tensor,
                tail: torch.Tensor, block_table: torch.Tensor, slots: torch.Tensor, scale: float, rot: bool,
