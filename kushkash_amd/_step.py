@@ -68,10 +68,15 @@ def block_table(req_to_token: torch.Tensor, req: torch.Tensor, seq_lens: torch.T
     if dev.type != "cuda":
         n = seq_lens.long().clamp(max=req_to_token.shape[1])
         known = (req >= 0) & (req < req_to_token.shape[0])
-        at = torch.arange(pages, device=dev) * PAGE
-        ids = torch.div(req_to_token[torch.where(known, req, 0).long()][:, at.clamp(max=max(req_to_token.shape[1] - 1, 0))],
-                        PAGE, rounding_mode="floor") if req_to_token.numel() else torch.zeros(R, pages, dtype=torch.int32)
-        table.copy_(torch.where((at[None, :] < n[:, None]) & known[:, None], ids, 0))
+        first = req_to_token[:, ::PAGE][:, :pages]                  # each page's first token
+        cols = first.shape[1]
+        if first.numel():
+            seen = (torch.arange(cols) * PAGE < n[:, None]) & known[:, None]
+            ids = torch.div(first[torch.where(known, req, 0).long()], PAGE, rounding_mode="floor")
+            table[:, :cols].copy_(torch.where(seen, ids, 0))
+        else:
+            cols = 0
+        table[:, cols:].zero_()
         lens.copy_(seq_lens)
         slots.copy_(req)
     elif R:
