@@ -107,6 +107,10 @@ class MapSizes:
         """The sizes without the maps that unpack history: of a step that only writes its tokens."""
         return replace(self, pages=0, tails=0)
 
+    def times(self, n: int) -> "MapSizes":
+        """The sizes of n steps of these one behind the other: of sequences of one length each."""
+        return MapSizes(*(n * x for x in self.numbers[:-2]), self.window, self.sinks)
+
 
 @dataclass
 class StepMaps:
