@@ -189,8 +189,6 @@ def prepare(c, seed):
             s["splits"] = ops.splits(c["batch"], c["hkv"], max(s["lens"]) // PAGE, window=c["window"], sinks=c["sinks"])
             s["work"] = torch.empty(c["batch"] * c["hkv"] * s["splits"] * c["group"] * (c["dim"] + 2),
                                     dtype=torch.float32, device="cuda")
-        if c["kind"] == "maps":
-            s["sizes"] = kk.map_sizes(s["T"], s["H"], **s["limit"])
     return s
 
 
@@ -286,7 +284,8 @@ def run(s):
         if c["kind"] == "table":
             return kk.block_table(s["req_to_token"], s["req"], s["seq_lens"], s["pages"])
         if c["kind"] == "maps":
-            m = kk.step_maps(s["new"], s["history"], s["slots"], s["table"], s["sizes"])
+            # (the lengths are another step's every time, so their sizes are part of the pass, as in the plain form)
+            m = kk.step_maps(s["new"], s["history"], s["slots"], s["table"], kk.map_sizes(s["T"], s["H"], **s["limit"]))
             return [getattr(m, name) for name in MAPS]
         return kk.sample(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"], min_p=s["min_p"])
     return PLAIN[c["kind"]](s, c)
