@@ -31,6 +31,7 @@ import torch
 from ._window import PAGE, check_limit
 
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+NO_WINDOW = "a window is a GPU extension; the CPU path attends over every token"
 DECODE_WAVES = 4                # default waves per decode workgroup (kush_decode: waves = 0)
 SYNC_SLOTS = 1 << 16            # split-K merge counters per Ops: (sequence, kv head, 16-head chunk) slots
 
@@ -517,6 +518,7 @@ class Ops:
         decode. No reference counterpart."""
         window, sinks = check_limit(window, sinks)
         limit = {"window": window, "sinks": sinks} if window else {}
+        _require(self.gpu or not window, NO_WINDOW)                       # before the append
         if window and self._native_window(k, v, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work,
                                           waves, order, rot, window, sinks):
             return
@@ -556,7 +558,7 @@ class Ops:
         if n_splits < 1:
             raise ValueError("n_splits must be >= 1")
         self._check_values(cache, block_table, seq_lens, tail_idx, tail_k, S, window=window, sinks=sinks)
-        _require(self.gpu or not window, "a window is a GPU extension; the CPU path attends over every token")
+        _require(self.gpu or not window, NO_WINDOW)
         if not self.gpu:                # one pass per (sequence, kv head): splits, work, waves, order unused
             _require(not rot, "decode(rot=True) is a GPU extension; the CPU path takes a rotated q (fwht)")
             bs, hs = _byte_strides(cache)
