@@ -105,8 +105,9 @@ def plan(spans, group: int, hkv: int, D: int, total_q: int, causal: bool = True,
                than min(scratch, PARTIAL_BYTES) holds the partials of.
     With a window a row tile's keys are those that it sees, wherever they lie. Below 24 tiles, where the row tiles leave
                half the chip idle, they are split as well, into parts of 3 tiles and more, if the tiles saved take
-               longer than the merge's launch and bytes (24 row tiles of 10 key tiles: 27.1 us whole, 21.5 in four; 3
-               of 14: 23.9, in five 16.1; 12 of 7: 15.0, in two 17.0; 144 of 7: 22.4, 28.2)."""
+               longer than the merge's launch and bytes (D 128, times with the launch, q and the store, ~8 us: 24 row tiles
+               of 10 key tiles 27.1 us whole, 21.5 in four; 3 of 14 23.9, in five 16.1; 12 of 7 15.0, in two 17.0; 144 of 7
+               22.4, 28.2)."""
     longest = max([n for _, n, _ in spans])
     if window:
         longest = min(longest, window_tiles(window, sinks, 128, group) * KEYS)

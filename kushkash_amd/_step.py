@@ -1,7 +1,7 @@
 """What surrounds the attention of a serving step, on the GPU kernels of csrc/kush_step.hip (include/kushkash_amd_step.h):
 its index arrays -- a decode step's block table, a prefill step's maps -- built from the requests' lengths, and the next
 tokens, drawn from the logits and given random numbers. On other devices block_table and step_maps are torch operations
-of the same results (what the serving integrations' host path runs on); sample is for the GPU."""
+of the same results (the serving integrations' host path runs on block_table; its maps are numpy's); sample is for the GPU."""
 from __future__ import annotations
 
 from dataclasses import dataclass, replace

@@ -147,7 +147,9 @@ __global__ __launch_bounds__(256) void step_maps_kernel(const MapArgs a) {
 // What it has to read is the logits, once; the passes read them three times, the later ones from the caches. One row of
 // 152,000 bf16 with top-k 50 and top-p takes 20 us (4, 5, 5 and 6: the launches' own times and the steps of one workgroup
 // over the list), 64 fp32 rows 47 (9, 11, 13 and 14: 39 MB, 8 us at the card's copy rate).
-// A list of more than LIST tokens (thousands of equal logits next to a cut) is cut by a radix search over the row instead.
+// A list of more than LIST tokens is cut by a radix search over the row instead, in one workgroup: thousands of equal logits next
+// to a cut, or fewer logits above -inf than top_k, which brings every masked token of the row into the list. Of 152,000 tokens
+// 20 allowed, top_k 50: one row 1.8 ms, 64 rows 2.2, with top-p 2.5 and 3.5 (all allowed: 20 and 38 us).
 struct SampleArgs {
     const void* logits;
     int64_t stride;
